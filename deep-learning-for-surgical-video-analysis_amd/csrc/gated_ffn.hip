@@ -1,0 +1,475 @@
+// Gated feed-forward block (svk_gated_ffn): both projections, the activation and the product in one kernel
+//
+//   h[m, c] = act(sum_k x[m, k] Wg[c, k] + bg[c]) * (sum_k x[m, k] Wu[c, k] + bu[c])
+//
+// and its backward pass.  The two weight matrices are one stacked [2H, K] (gate rows, then up rows).  The B rows of a
+// tile are taken alternately from the two halves, so that a wave's accumulators hold the gate and the up value of the
+// same (m, c) in the same lane: the product is formed in f32 registers, and the [M, 2H] projections never exist in
+// memory unless the caller keeps them for the backward pass (rounded to the storage type, once).
+//
+// Backward, from the kept projections g, u and dh:
+//   dg = dh u act'(g),  du = dh act(g)   (gated_dpre: f32, rounded once to the storage type: operands of the products;
+//                                         the bias gradient sums the unrounded values in f32)
+//   dx = [dg | du] [Wg; Wu],  dW = [dg | du]^T x   (tile_mm.h, col operands: no transposed copies)
+// Every sum has a fixed order: results do not change from run to run.
+#include "tile_mm.h"
+#include <algorithm>
+#include <type_traits>
+
+namespace svk {
+namespace gf {
+using namespace mm;
+
+// act(g); 16-bit results take the short forms (errors ~1e-7, far under half a step of either type)
+template <typename T>
+__device__ __forceinline__ float glu_act(float g, int act) {
+  if (act == SVK_GLU_SILU) {
+    if constexpr (sizeof(T) == 4) return g / (1.0f + expf(-g));
+    else return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+  }
+  if (act == SVK_GLU_GELU) {
+    if constexpr (sizeof(T) == 4) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    else return gelu_fast(g);
+  }
+  return g > 0.f ? g : (g <= 0.f ? 0.f : g);     // NaN stays NaN
+}
+// act(g) and act'(g)
+template <typename T>
+__device__ __forceinline__ void glu_grad(float g, int act, float& a, float& d) {
+  if (act == SVK_GLU_SILU) {
+    float s;
+    if constexpr (sizeof(T) == 4) s = 1.0f / (1.0f + expf(-g));
+    else s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+    a = g * s;
+    d = s * (1.0f + g * (1.0f - s));
+  } else if (act == SVK_GLU_GELU) {
+    const float p = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    a = g * p;
+    d = p + g * 0.3989422804014327f * expf(-0.5f * g * g);
+  } else {
+    a = g > 0.f ? g : (g <= 0.f ? 0.f : g);
+    d = g > 0.f ? 1.f : 0.f;
+  }
+}
+
+// 4 consecutive values of a row as one store (V4), or those that exist one by one
+template <typename T>
+__device__ __forceinline__ void put4(T* at, const float* v, int n, bool v4) {
+  T o[4] = {from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};
+  if (v4 && n >= 4) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) at[e] = o[e];
+  }
+}
+
+template <typename T>
+struct GateEpi {
+  T* h; long ldh;
+  T* pre;                 // [M, 2H] contiguous, or null
+  const float* bias;      // [2H] or null
+  int M, H, act;
+  bool v4, p4;            // 4-value stores of h / of pre are aligned
+
+  template <class C> __device__ __forceinline__ int row(int r, int tn) const {
+    const int w = r / C::WN, in = r % C::WN, up = in >= C::WN / 2;
+    const int c = tn * (C::BN / 2) + w * (C::WN / 2) + in - up * (C::WN / 2);
+    return min(c, H - 1) + up * H;
+  }
+  __device__ __forceinline__ int skinny_row(int bid, int j, int fr) const { return min(bid * 16 + fr, H - 1) + j * H; }
+  __device__ __forceinline__ void skinny_write(int bid, int m, int n, float g, float u) const {
+    const int c = bid * 16 + n;
+    if (c >= H) return;
+    if (bias) {
+      g += bias[c];
+      u += bias[H + c];
+    }
+    if (pre) {
+      pre[(long)m * 2 * H + c] = from_f<T>(g);
+      pre[(long)m * 2 * H + H + c] = from_f<T>(u);
+    }
+    h[(long)m * ldh + c] = from_f<T>(glu_act<T>(g, act) * u);
+  }
+  template <class C, typename A>
+  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
+    constexpr int TG = C::TN / 2;
+    static_assert(C::TN % 2 == 0, "a wave's columns are half gate, half up");
+#pragma unroll
+    for (int j = 0; j < TG; ++j) {
+      const int c = tn * (C::BN / 2) + wn * (C::WN / 2) + j * 16 + fq * 4, left = H - c;
+      if (left <= 0) continue;
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) {
+            bg[e] = bias[c + e];
+            bu[e] = bias[H + c + e];
+          }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int m = m0 + i * 16;
+        if (m >= M) continue;
+        float g[4], u[4], o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = acc[i][j][e] + bg[e];
+          u[e] = acc[i][j + TG][e] + bu[e];
+          o[e] = glu_act<T>(g[e], act) * u[e];
+        }
+        if (pre) {
+          put4<T>(pre + (long)m * 2 * H + c, g, left, p4);
+          put4<T>(pre + (long)m * 2 * H + H + c, u, left, p4);
+        }
+        put4<T>(h + (long)m * ldh + c, o, left, v4);
+      }
+    }
+  }
+};
+
+// plain product: rounded to T, or an f32 slab of one part of the reduction
+template <typename T>
+struct PlainEpi {
+  T* y; long ldy;
+  float* slab;            // [parts][M][N], or null
+  int M, N;
+  bool v4, s4;
+  template <class C> __device__ __forceinline__ int row(int r, int tn) const { return min(tn * C::BN + r, N - 1); }
+  template <class C, typename A>
+  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = tn * C::BN + wn * C::WN + j * 16 + fq * 4, left = N - n;
+      if (left <= 0) continue;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int m = m0 + i * 16;
+        if (m >= M) continue;
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (slab) put4<float>(slab + ((long)blockIdx.y * M + m) * N + n, v, left, s4);
+        else put4<T>(y + (long)m * ldy + n, v, left, v4);
+      }
+    }
+  }
+};
+
+// y[m][n] = sum of the parts' slabs, in order
+template <typename T>
+__global__ __launch_bounds__(256) void join_parts(const float* __restrict__ S, int parts, T* __restrict__ y, long ldy, int M,
+                                                  int N) {
+  const long total = (long)M * N;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    float v = 0.f;
+    for (int s = 0; s < parts; ++s) v += S[s * total + i];
+    const long m = i / N;
+    y[m * ldy + (i - m * N)] = from_f<T>(v);
+  }
+}
+
+// dg, du from the kept projections: D [M][ld] = dg | du | zeros up to ld; S [row blocks][2H] = their column sums over
+// a block of rows, f32, before the rounding.  4 waves a workgroup, 64 * V columns, rows dealt to the waves in turn.
+constexpr int DP_ROWS = 64;
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, const T* __restrict__ dh, long lddh,
+                                                  T* __restrict__ D, long ld, float* __restrict__ S, int M, int H, int act) {
+  __shared__ float sum[2][4][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (blockIdx.y * 64 + lane) * V;
+  const long r0 = (long)blockIdx.x * DP_ROWS, r1 = min(r0 + DP_ROWS, (long)M);
+  const int nc = H - c;                       // columns that exist from c on (V divides H where V > 1)
+  float sg[V], su[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sg[e] = su[e] = 0.f;
+  typedef T vec __attribute__((ext_vector_type(V)));
+  for (long r = r0 + wave; r < r1; r += 4) {
+    if (nc > 0) {
+      const vec g = *reinterpret_cast<const vec*>(pre + r * 2 * H + c), u = *reinterpret_cast<const vec*>(pre + r * 2 * H + H + c);
+      const vec d = *reinterpret_cast<const vec*>(dh + r * lddh + c);
+      vec og, ou;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float a, da;
+        glu_grad<T>(to_f(g[e]), act, a, da);
+        const float dg = to_f(d[e]) * to_f(u[e]) * da, du = to_f(d[e]) * a;
+        og[e] = from_f<T>(dg);
+        ou[e] = from_f<T>(du);
+        sg[e] += dg;
+        su[e] += du;
+      }
+      *reinterpret_cast<vec*>(D + r * ld + c) = og;
+      *reinterpret_cast<vec*>(D + r * ld + H + c) = ou;
+    }
+    // the padding of the row, by the last column block
+    if (blockIdx.y == gridDim.y - 1 && 2 * H + lane < ld) D[r * ld + 2 * H + lane] = from_f<T>(0.f);
+  }
+  if (!S) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    sum[0][wave][lane * V + e] = sg[e];
+    sum[1][wave][lane * V + e] = su[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * 64 * V; i += 256) {
+    const int half = i / (64 * V), k = i % (64 * V), col = blockIdx.y * 64 * V + k;
+    if (col < H) S[(long)blockIdx.x * 2 * H + half * H + col] = (sum[half][0][k] + sum[half][1][k]) + (sum[half][2][k] + sum[half][3][k]);
+  }
+}
+
+// db[c] = sum of the row blocks' sums, in order: 16 columns a workgroup, 16 threads a column
+__global__ __launch_bounds__(256) void join_bias(const float* __restrict__ S, int blocks, float* __restrict__ db, int N) {
+  __shared__ float part[16][17];
+  const int cl = threadIdx.x & 15, t = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float v = 0.f;
+  if (c < N)
+    for (int b = t; b < blocks; b += 16) v += S[(long)b * N + c];
+  part[t][cl] = v;
+  __syncthreads();
+  if (t == 0 && c < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += part[i][cl];
+    db[c] = s;
+  }
+}
+
+using Big = Tile<256, 256, 2, 4, 2, 2>;
+using Mid = Tile<128, 128, 2, 2, 2, 2>;
+using Small = Tile<64, 64, 2, 2, 4, 2>;
+
+// tile choice: the largest tile that still gives the chip's 256 CUs most of a workgroup each
+inline int pick(long m, long n, long parts = 1) {
+  auto tiles = [&](long b) { return ((m + b - 1) / b) * ((n + b - 1) / b) * parts; };
+  if (tiles(256) >= 200) return 0;
+  if (tiles(128) >= 200) return 1;
+  return 2;
+}
+
+template <typename T, class C, bool AC, bool BC, class Epi>
+static int go(Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
+  p.ntm = (int)((m + C::BM - 1) / C::BM);
+  p.ntn = (int)((n + C::BN - 1) / C::BN);
+  if ((long)p.ntm * p.ntn > 0x7fffffffL) { set_error("%s: too many tiles", name); return SVK_EUNSUPPORTED; }
+  hipLaunchKernelGGL((tile_mm<T, C, AC, BC, Epi>), dim3(p.ntm * p.ntn, p.parts), dim3(C::NT), 0, st, p, epi);
+  set_last_kernel(name);
+  return check_launch(name);
+}
+template <typename T, bool AC, bool BC, class Epi>
+static int tiled(int cfg, Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
+  p.nk = (p.K + 128 / (int)sizeof(T) - 1) / (128 / (int)sizeof(T));
+  if (cfg == 0) return go<T, Big, AC, BC>(p, m, n, epi, st, name);
+  if (cfg == 1) return go<T, Mid, AC, BC>(p, m, n, epi, st, name);
+  return go<T, Small, AC, BC>(p, m, n, epi, st, name);
+}
+
+template <typename T, int MT, class Epi>
+static int skinny_mt(const Args& p, bool vec, int blocks, const Epi& epi, hipStream_t st) {
+  if (vec) hipLaunchKernelGGL((skinny_mm<T, MT, true, Epi>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
+  else hipLaunchKernelGGL((skinny_mm<T, MT, false, Epi>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
+  set_last_kernel("skinny_mm");
+  return check_launch("skinny_mm");
+}
+
+constexpr int SKINNY_M = 32;
+
+// the weight gradient's split of the token axis: small outputs would leave most CUs idle over a long reduction
+inline int dw_parts(long n2, long k, long m, int bk) {
+  const long tiles = ((n2 + 127) / 128) * ((k + 127) / 128);
+  const long nk = (m + bk - 1) / bk;
+  long parts = std::min<long>((512 + tiles - 1) / tiles, nk / 8);
+  parts = std::max<long>(1, std::min<long>(parts, 64));
+  const long per = (nk + parts - 1) / parts;
+  return (int)((nk + per - 1) / per);          // no empty part
+}
+
+// workspace of the backward pass: [dpre][x padded][w padded][bias partials][dw slabs]
+struct BwdWs {
+  long ldd, dpre, x, w, sums, slabs, total;
+  int parts;
+  BwdWs(long es, long M, long H, long K, bool padx, bool db, bool dw) {
+    ldd = up16(2 * H * es) / es;
+    dpre = up16(M * ldd * es);
+    const long ldk = up16(K * es);
+    x = padx ? up16(M * ldk) : 0;
+    w = padx ? up16(2 * H * ldk) : 0;
+    sums = db ? up16((M + DP_ROWS - 1) / DP_ROWS * 2 * H * 4) : 0;
+    parts = dw ? dw_parts(2 * H, K, M, 128 / (int)es) : 1;
+    slabs = parts > 1 ? up16(parts * 2 * H * K * 4) : 0;
+    total = dpre + x + w + sums + slabs;
+  }
+};
+
+static bool bad_dims(long M, long H, long K) {
+  // 32-bit row and column counts inside a kernel; 65535 column blocks of gated_dpre
+  return M < 0 || H <= 0 || K <= 0 || M > 0x7fffff00L || H > 4000000L || K > 0x1fffff00L;
+}
+
+template <typename T>
+static int pad(const void* X, long ldx, void* Y, long rows, long K, hipStream_t st) {
+  const long ld = up16(K * (long)sizeof(T)) / (long)sizeof(T);
+  const long blocks = std::min<long>((rows * ld + 255) / 256, 8192);
+  hipLaunchKernelGGL((pad_rows<T>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)X, ldx, (T*)Y, ld, rows, (int)K);
+  return check_launch("pad_rows");
+}
+
+static int es_of(int dtype) { return dtype == SVK_F32 ? 4 : (dtype == SVK_BF16 || dtype == SVK_F16 ? 2 : 0); }
+
+}  // namespace gf
+}  // namespace svk
+
+using namespace svk;
+using namespace svk::gf;
+
+// rows that the tiled kernels can read as they are
+static bool rows_ok(const void* p, long ld, long width, long es) { return al16(p) && ld * es % 16 == 0 && width * es % 16 == 0; }
+
+extern "C" long svk_gated_ffn_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K) {
+  const long es = es_of(dtype);
+  if (!es || bad_dims(M, H, K) || M <= SKINNY_M) return 0;
+  const long ldk = up16(K * es);
+  return (rows_ok(X, ldx, K, es) ? 0 : M * ldk) + (rows_ok(W, ldw, K, es) ? 0 : 2 * H * ldk);
+}
+
+extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, long ldw, const float* bias, void* Hout,
+                             long ldh, void* pre, long M, long H, long K, int act, void* ws, long ws_bytes, void* stream) {
+  const long es = es_of(dtype);
+  if (!es) { set_error("svk_gated_ffn: unsupported dtype %d", dtype); return SVK_EINVAL; }
+  if (!X || !W || !Hout || bad_dims(M, H, K) || ldx < K || ldw < K || ldh < H || act < SVK_GLU_SILU || act > SVK_GLU_RELU) {
+    set_error("svk_gated_ffn: bad args");
+    return SVK_EINVAL;
+  }
+  const long ldk = up16(K * es);
+  if (2 * H * std::max(ldw * es, ldk) >= (1L << 32) || 256 * std::max(ldx * es, ldk) >= (1L << 32)) {
+    set_error("svk_gated_ffn: weights or 256 rows of x of 4 GiB or more");
+    return SVK_EUNSUPPORTED;
+  }
+  if (ws_bytes < svk_gated_ffn_workspace(dtype, X, ldx, W, ldw, M, H, K)) { set_error("svk_gated_ffn: workspace too small"); return SVK_EINVAL; }
+  if (M == 0) return SVK_OK;
+  hipStream_t st = (hipStream_t)stream;
+  SVK_DISPATCH_DTYPE(dtype, T, {
+    GateEpi<T> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, false, false};
+    epi.v4 = H % 4 == 0 && ldh % 4 == 0 && ((uintptr_t)Hout & (4 * es - 1)) == 0;
+    epi.p4 = H % 4 == 0 && ((uintptr_t)pre & (4 * es - 1)) == 0;
+    Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, (int)M, (int)(2 * H), (int)K, 0, 0, 0, 1};
+    if (M <= SKINNY_M) {
+      const bool vec = rows_ok(X, ldx, K, es) && rows_ok(W, ldw, K, es);
+      const int blocks = (int)((H + 15) / 16);
+      return M <= 16 ? skinny_mt<T, 1>(p, vec, blocks, epi, st) : skinny_mt<T, 2>(p, vec, blocks, epi, st);
+    }
+    char* at = (char*)ws;
+    if (!rows_ok(X, ldx, K, es)) {
+      if (int rc = pad<T>(X, ldx, at, M, K, st)) return rc;
+      p.A = at;
+      p.lda = ldk;
+      at += M * ldk;
+      p.K = (int)(ldk / es);
+    }
+    if (!rows_ok(W, ldw, K, es)) {
+      if (int rc = pad<T>(W, ldw, at, 2 * H, K, st)) return rc;
+      p.B = at;
+      p.ldb = ldk;
+      p.K = (int)(ldk / es);
+    }
+    return tiled<T, false, false>(pick(M, 2 * H), p, M, 2 * H, epi, st, "gated_ffn");
+  });
+}
+
+extern "C" long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H,
+                                            long K, int want_dw, int want_db) {
+  const long es = es_of(dtype);
+  if (!es || bad_dims(M, H, K) || M == 0) return 0;
+  const bool padx = !rows_ok(X, ldx, K, es) || !rows_ok(W, ldw, K, es);
+  return BwdWs(es, M, H, K, padx, want_db, want_dw).total;
+}
+
+extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre,
+                                 const void* dH, long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K,
+                                 int act, void* ws, long ws_bytes, void* stream) {
+  const long es = es_of(dtype);
+  if (!es) { set_error("svk_gated_ffn_bwd: unsupported dtype %d", dtype); return SVK_EINVAL; }
+  if (!X || !W || !pre || !dH || bad_dims(M, H, K) || ldx < K || ldw < K || lddh < H || (dX && lddx < K) ||
+      act < SVK_GLU_SILU || act > SVK_GLU_RELU) {
+    set_error("svk_gated_ffn_bwd: bad args");
+    return SVK_EINVAL;
+  }
+  const long ldk = up16(K * es);
+  if (256 * std::max(std::max(ldx, ldw) * es, std::max(ldk, up16(2 * H * es))) >= (1L << 32)) {
+    set_error("svk_gated_ffn_bwd: 256 rows of 4 GiB or more");
+    return SVK_EUNSUPPORTED;
+  }
+  const bool padx = !rows_ok(X, ldx, K, es) || !rows_ok(W, ldw, K, es);
+  const BwdWs need(es, M, H, K, padx, db, dW);
+  if (M && (!ws || !al16(ws) || ws_bytes < need.total)) { set_error("svk_gated_ffn_bwd: workspace too small or misaligned"); return SVK_EINVAL; }
+  hipStream_t st = (hipStream_t)stream;
+  SVK_DISPATCH_DTYPE(dtype, T, {
+    if (M == 0) {                                   // no tokens: the sums are empty
+      if (dW) {
+        hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((2 * H * K + 255) / 256, 8192)), dim3(256), 0, st, nullptr, 0, (T*)dW, K, (int)(2 * H), (int)K);
+        if (int rc = check_launch("join_parts")) return rc;
+      }
+      if (db) {
+        hipLaunchKernelGGL(join_bias, dim3((unsigned)((2 * H + 15) / 16)), dim3(256), 0, st, nullptr, 0, db, (int)(2 * H));
+        return check_launch("join_bias");
+      }
+      return SVK_OK;
+    }
+    char* at = (char*)ws;
+    T* D = (T*)at;
+    at += need.dpre;
+    Args px{(const char*)X, nullptr, ldx * es, 0, 0, 0, 0, 0, 0, 0, 1};
+    const char* Wr = (const char*)W;
+    long ldwb = ldw * es;
+    if (padx) {
+      if (int rc = pad<T>(X, ldx, at, M, K, st)) return rc;
+      px.A = at;
+      px.lda = ldk;
+      at += need.x;
+      if (int rc = pad<T>(W, ldw, at, 2 * H, K, st)) return rc;
+      Wr = at;
+      ldwb = ldk;
+      at += need.w;
+    }
+    float* sums = db ? (float*)at : nullptr;
+    at += need.sums;
+    float* slabs = need.parts > 1 ? (float*)at : nullptr;
+    const int rowblocks = (int)((M + DP_ROWS - 1) / DP_ROWS);
+    constexpr int V = 16 / (int)sizeof(T);
+    auto al = [&](const void* q) { return ((uintptr_t)q & 15) == 0; };
+    if (H % V == 0 && lddh % V == 0 && al(pre) && al(dH)) {
+      hipLaunchKernelGGL((gated_dpre<T, V>), dim3(rowblocks, (unsigned)((H + 64 * V - 1) / (64 * V))), dim3(256), 0, st,
+                         (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act);
+    } else {
+      hipLaunchKernelGGL((gated_dpre<T, 1>), dim3(rowblocks, (unsigned)((H + 63) / 64)), dim3(256), 0, st, (const T*)pre,
+                         (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act);
+    }
+    if (int rc = check_launch("gated_dpre")) return rc;
+    if (db) {
+      hipLaunchKernelGGL(join_bias, dim3((unsigned)((2 * H + 15) / 16)), dim3(256), 0, st, sums, rowblocks, db, (int)(2 * H));
+      if (int rc = check_launch("join_bias")) return rc;
+    }
+    if (dX) {
+      PlainEpi<T> epi{(T*)dX, lddx, nullptr, (int)M, (int)K, false, false};
+      epi.v4 = lddx % 4 == 0 && ((uintptr_t)dX & (4 * es - 1)) == 0;
+      // the padding of D is zero and rows of W past 2H read as zero, so the reduction runs over whole chunks
+      Args p{(const char*)D, Wr, need.ldd * es, ldwb, (int)M, (int)K, (int)(2 * H), 0, 0, 0, 1};
+      if (int rc = tiled<T, false, true>(pick(M, K), p, M, K, epi, st, "gated_ffn_dx")) return rc;
+    }
+    if (dW) {
+      PlainEpi<T> epi{(T*)dW, K, slabs, (int)(2 * H), (int)K, false, false};
+      epi.v4 = K % 4 == 0 && ((uintptr_t)dW & (4 * es - 1)) == 0;
+      epi.s4 = K % 4 == 0;
+      Args p{(const char*)D, px.A, need.ldd * es, px.lda, (int)(2 * H), (int)K, (int)M, 0, 0, 0, need.parts};
+      const int cfg = need.parts > 1 ? 1 : pick(2 * H, K);
+      if (int rc = tiled<T, true, true>(cfg, p, 2 * H, K, epi, st, "gated_ffn_dw")) return rc;
+      if (slabs) {
+        const long total = 2 * H * K;
+        hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((total + 255) / 256, 8192)), dim3(256), 0, st, slabs,
+                           need.parts, (T*)dW, K, (int)(2 * H), (int)K);
+        return check_launch("join_parts");
+      }
+    }
+    return SVK_OK;
+  });
+}

@@ -112,6 +112,14 @@ SIGNATURES = {
     "svk_pack_params": [c_int, P, c_int, c_long, P, P, P],
     "svk_pack_params8": [c_int, P, c_int, c_long, P, P, P],
     "svk_pack_transpose": [c_int, P, c_int, P, P, P],
+    "svk_rope3d": [c_int, P, c_long, c_long, P, c_long, c_long, c_int, P, c_long, c_long, P, c_long, c_long, c_int, P,
+                   c_int, c_long, c_long, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
+    "svk_gated_ffn": [c_int, P, c_long, P, c_long, P, P, c_long, P, c_long, c_long, c_long, c_int, P, c_long, P],
+    "svk_gated_ffn_bwd": [c_int, P, c_long, P, c_long, P, P, c_long, P, c_long, P, P, c_long, c_long, c_long, c_int, P,
+                          c_long, P],
+    "svk_quant_rows": [c_int, P, c_long, P, c_long, P, c_long, c_long, P],
+    "svk_gemm_i8": [c_int, P, c_long, P, P, c_long, P, P, P, c_long, P, c_long, c_long, c_long, c_long, c_int, P, c_long,
+                    P],
 }
 STRING_FUNCS = ("svk_version", "svk_last_error", "svk_last_kernel")
 LONG_FUNCS = {"svk_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int, c_int],
@@ -122,7 +130,10 @@ LONG_FUNCS = {"svk_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int,
               "svk_mamba_scan_bwd_workspace": [c_int, c_int, c_int, c_int],
               "svk_mamba_scan_ragged_workspace": [c_int, c_int, c_int],
               "svk_mstcn_bwd_workspace": [c_int, c_int],
-              "svk_stats_ws_floats": [c_int, c_int]}
+              "svk_stats_ws_floats": [c_int, c_int],
+              "svk_gated_ffn_workspace": [c_int, P, c_long, P, c_long, c_long, c_long, c_long],
+              "svk_gated_ffn_bwd_workspace": [c_int, P, c_long, P, c_long, c_long, c_long, c_long, c_int, c_int],
+              "svk_gemm_i8_workspace": [P, c_long, P, c_long, c_long, c_long, c_long]}
 INT_QUERIES = {"svk_mixffn_supported": [c_int, c_int], "svk_mixffn_rw_supported": [c_int, c_int, c_int],
                "svk_mixffn_dw_fc2_supported": [c_int, c_int, c_int, c_int],
                "svk_conv2d_s2d_ln_supported": [c_int, c_int, c_int, c_int], "svk_mstcn_tile_size": []}

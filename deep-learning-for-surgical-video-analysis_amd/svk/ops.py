@@ -1474,3 +1474,281 @@ def adamw(p, g, m, v, lr, step, partials=None, max_norm=0.0, beta1=0.9, beta2=0.
 def mstcn_bwd_floats(T, F):
     """f32 count of the svk_mstcn_layer_bwd workspace for a [T, F] layer."""
     return _lib.load().svk_mstcn_bwd_workspace(T, F) // 4
+
+
+# ---- token-block operators: rotary positions over (time, height, width), gated feed-forward, 8-bit products
+
+GLU_ACT = {"silu": 0, "gelu": 1, "relu": 2}
+_POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _same_device(fn, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise _lib.SvkError(f"svk.{fn}: tensors on {first.device} and {t.device}")
+
+
+def _on(first, name, *args):
+    """The library call on ``first``'s device and that device's current stream."""
+    i = first.device.index
+    if i == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(i):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _token_rows(t, fn, name):
+    """(rows, columns, row stride) of a [..., C] tensor whose leading dims are one even run of rows; dims of one
+    element do not count (the newest token x[:, -1:] of a batch is such a run)."""
+    cols = t.shape[-1] if t.dim() else 0
+    if cols == 0 or (cols > 1 and t.stride(-1) != 1):
+        raise _lib.SvkError(f"svk.{fn}: {name} {tuple(t.shape)} must have a last dim of unit stride")
+    rows, ld, run = t.numel() // cols, None, None
+    if rows > 1:
+        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if ld is None:
+                ld = run = s
+            elif s != run:
+                raise _lib.SvkError(f"svk.{fn}: {name} leading dims are not uniformly strided")
+            run *= n
+    ld = cols if ld is None else ld
+    if rows > 1 and ld < cols:
+        raise _lib.SvkError(f"svk.{fn}: {name} rows overlap (stride {ld} < {cols} columns)")
+    return rows, cols, ld
+
+
+def _vector(t, n, fn, name):
+    if t is not None:
+        _chk(t, name, torch.float32)
+        if t.numel() != n or not t.is_contiguous():
+            raise _lib.SvkError(f"svk.{fn}: {name} must be {n} contiguous float32 values, got {tuple(t.shape)}")
+
+
+def _apart(a, b):
+    """False where writing ``a`` may change ``b``: their memory meets, and they are not the same elements in the same
+    order, nor two column ranges of one buffer's rows."""
+    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
+        return True
+    ea, eb = a.element_size(), b.element_size()
+    last = lambda t, e: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * e  # noqa: E731
+    if last(a, ea) <= b.data_ptr() or last(b, eb) <= a.data_ptr():
+        return True
+    if ea != eb:
+        return False
+    if a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride():
+        return True
+    if a.dim() == b.dim() and a.shape[:-1] == b.shape[:-1] and a.stride() == b.stride() and a.dim() > 1:
+        ld = min((s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1), default=0)
+        if ld and all(s % ld == 0 for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1):
+            d = (b.data_ptr() - a.data_ptr()) // ea % ld
+            return a.shape[-1] <= d and d + b.shape[-1] <= ld
+    return False
+
+
+def rope3d_freqs(sections, base=10000.0, shared=False, device="cuda"):
+    """Radians a step of the R = sum(sections) rotary pairs, float64 [R], for ``rope3d``: pair j of an axis with n
+    pairs turns by base ** (-j / n); with ``shared`` the axes divide one series base ** (-i / R) instead."""
+    if len(sections) != 3 or min(sections) < 0 or sum(sections) < 1:
+        raise _lib.SvkError(f"svk.rope3d_freqs: sections {tuple(sections)} must be three counts of pairs")
+    if shared:
+        e = torch.arange(sum(sections), dtype=torch.float64) / sum(sections)
+    else:
+        e = torch.cat([torch.arange(n, dtype=torch.float64) / max(n, 1) for n in sections])
+    return torch.pow(torch.tensor(float(base), dtype=torch.float64), -e).to(device)
+
+
+def rope3d(q, k, pos, freqs, sections, heads, kv_heads=None, interleaved=False, inverse=False, out=None):
+    """(q', k') with every head's pairs turned by the token's (time, row, column): svk_rope3d.
+
+    q [B, N, heads * hd], k [B, N, kv_heads * hd] or None (any row / batch strides, unit channel stride); pos [N, 3] or
+    [B, N, 3] int32 / int64 / float32; sections = pairs of the three axes, in this order, 2 * sum <= hd; freqs float64
+    [sum(sections)] (rope3d_freqs).  ``inverse`` turns back: the gradient of the rotation.  ``out`` = (q', k') to write,
+    which may be (q, k)."""
+    fn = "rope3d"
+    dt = dtype_code(q.dtype)
+    _chk(q, "q"); _chk(k, "k", q.dtype); _chk(pos, "pos"); _chk(freqs, "freqs", torch.float64)
+    kv_heads = 0 if k is None else heads if kv_heads is None else kv_heads
+    nt, nh, nw = sections
+    if q.dim() != 3 or heads < 1 or q.shape[2] % heads or q.shape[2] == 0:
+        raise _lib.SvkError(f"svk.rope3d: q {tuple(q.shape)} is not [B, N, {heads} * hd]")
+    B, N, C = q.shape
+    hd = C // heads
+    if k is not None and (kv_heads < 1 or k.shape != (B, N, kv_heads * hd)):
+        raise _lib.SvkError(f"svk.rope3d: k {tuple(k.shape)} is not [{B}, {N}, {kv_heads} * {hd}]")
+    if min(nt, nh, nw) < 0 or not 0 < 2 * (nt + nh + nw) <= hd:
+        raise _lib.SvkError(f"svk.rope3d: sections {tuple(sections)} do not fit a head of {hd}")
+    if freqs.shape != (nt + nh + nw,) or not freqs.is_contiguous():
+        raise _lib.SvkError(f"svk.rope3d: freqs must be {nt + nh + nw} contiguous float64 values")
+    if pos.dtype not in _POS or pos.shape not in ((N, 3), (B, N, 3)) or pos.stride(-1) != 1:
+        raise _lib.SvkError(f"svk.rope3d: pos must be [N, 3] or [B, N, 3] int32 / int64 / float32 of unit stride, got "
+                            f"{tuple(pos.shape)} {pos.dtype}")
+    if out is None:
+        qo = torch.empty(B, N, C, device=q.device, dtype=q.dtype)
+        ko = None if k is None else torch.empty(B, N, kv_heads * hd, device=q.device, dtype=q.dtype)
+    else:
+        qo, ko = out
+        if (ko is None) != (k is None):
+            raise _lib.SvkError("svk.rope3d: out must be (q', k') like (q, k)")
+        for o, t, nm in ((qo, q, "q"), (ko, k, "k")):
+            if t is None:
+                continue
+            _chk(o, "out", q.dtype)
+            if o.shape != t.shape:
+                raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
+            width = t.shape[2]
+            if (N > 1 and o.stride(1) < width) or (B > 1 and o.stride(0) < (o.stride(1) * (N - 1) if N > 1 else 0) + width):
+                raise _lib.SvkError("svk.rope3d: out rows overlap")
+        if not (_apart(qo, q) and _apart(qo, k) and _apart(ko, k) and _apart(ko, q) and _apart(qo, ko)) or \
+                (ko is not None and qo.data_ptr() == ko.data_ptr() and qo.numel()):
+            raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
+    for t, nm in ((q, "q"), (k, "k"), (qo, "out"), (ko, "out")):
+        if t is not None and t.stride(2) != 1 and t.shape[2] > 1:
+            raise _lib.SvkError(f"svk.rope3d: {nm} must have unit channel stride")
+    _same_device(fn, q, k, pos, freqs, qo, ko)
+    if B * N:
+        s = lambda t: (None, 0, 0) if t is None else (t.data_ptr(), t.stride(1), t.stride(0))  # noqa: E731
+        _on(q, "svk_rope3d", dt, *s(q), *s(qo), heads, *s(k), *s(ko), kv_heads, pos.data_ptr(), _POS[pos.dtype],
+            pos.stride(-2), pos.stride(0) if pos.dim() == 3 else 0, freqs.data_ptr(), nt, nh, nw, hd, B, N,
+            int(interleaved), int(inverse))
+    return qo, ko
+
+
+def _glu(act, fn):
+    try:
+        return GLU_ACT[act]
+    except KeyError:
+        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(GLU_ACT)}") from None
+
+
+def _gated_args(x, w, fn):
+    dt = dtype_code(x.dtype)
+    _chk(x, "x"); _chk(w, "w", x.dtype)
+    M, K, ldx = _token_rows(x, fn, "x")
+    if w.dim() != 2 or w.shape[1] != K or w.shape[0] % 2 or w.shape[0] == 0:
+        raise _lib.SvkError(f"svk.{fn}: w {tuple(w.shape)} is not [2 * hidden, {K}] (gate rows, then up rows)")
+    _, _, ldw = _token_rows(w, fn, "w")
+    return dt, M, K, ldx, ldw, w.shape[0] // 2
+
+
+def _bytes(n, like):
+    return torch.empty(n, device=like.device, dtype=torch.uint8) if n else None
+
+
+def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
+    """act(x wg^T + bg) * (x wu^T + bu) in one kernel (svk_gated_ffn): x [..., K], w = cat([wg, wu]) [2 * hidden, K],
+    bias = cat([bg, bu]) float32 or None, act "silu" / "gelu" / "relu" -> [..., hidden].  ``save`` returns (h, pre) with
+    pre [..., 2 * hidden] the two projections, which gated_ffn_bwd reads.  The down projection is ``gemm``."""
+    fn = "gated_ffn"
+    dt, M, K, ldx, ldw, H = _gated_args(x, w, fn)
+    code = _glu(act, fn)
+    _vector(bias, 2 * H, fn, "bias")
+    lead = x.shape[:-1]
+    if out is None:
+        out, ldh = torch.empty(*lead, H, device=x.device, dtype=x.dtype), H
+    else:
+        _chk(out, "out", x.dtype)
+        if out.shape != (*lead, H):
+            raise _lib.SvkError(f"svk.{fn}: out is {tuple(out.shape)}, not {(*lead, H)}")
+        _, _, ldh = _token_rows(out, fn, "out")
+        if not (_apart(out, x) and _apart(out, w)) or (M and out.data_ptr() in (x.data_ptr(), w.data_ptr())):
+            raise _lib.SvkError(f"svk.{fn}: out overlaps an input")
+    pre = torch.empty(*lead, 2 * H, device=x.device, dtype=x.dtype) if save else None
+    _same_device(fn, x, w, bias, out)
+    if M:
+        px, pw = x.data_ptr(), w.data_ptr()
+        nb = _lib.load().svk_gated_ffn_workspace(dt, px, ldx, pw, ldw, M, H, K)
+        ws = _bytes(nb, x)
+        _on(x, "svk_gated_ffn", dt, px, ldx, pw, ldw, _p(bias), out.data_ptr(), ldh, _p(pre), M, H, K, code, _p(ws), nb)
+    return (out, pre) if save else out
+
+
+def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
+    """Gradients (dx, dw, db) of gated_ffn from dh [..., hidden] and the saved ``pre``: dx like x, dw [2 * hidden, K] in
+    w's dtype, db float32 [2 * hidden]; None where not asked for.  Written, not added to; the same bits on every run."""
+    fn = "gated_ffn_bwd"
+    dt, M, K, ldx, ldw, H = _gated_args(x, w, fn)
+    code = _glu(act, fn)
+    _chk(pre, "pre", x.dtype); _chk(dh, "dh", x.dtype)
+    lead = x.shape[:-1]
+    if pre.shape != (*lead, 2 * H) or not pre.is_contiguous():
+        raise _lib.SvkError(f"svk.{fn}: pre {tuple(pre.shape)} is not contiguous {(*lead, 2 * H)}")
+    if dh.shape != (*lead, H):
+        raise _lib.SvkError(f"svk.{fn}: dh {tuple(dh.shape)} is not {(*lead, H)}")
+    _, _, lddh = _token_rows(dh, fn, "dh")
+    _same_device(fn, x, w, pre, dh)
+    gx = torch.empty(*lead, K, device=x.device, dtype=x.dtype) if dx else None
+    gw = torch.empty(2 * H, K, device=x.device, dtype=x.dtype) if dw else None
+    gb = torch.empty(2 * H, device=x.device, dtype=torch.float32) if db else None
+    if (dx and M) or dw or db:
+        px, pw = x.data_ptr(), w.data_ptr()
+        nb = _lib.load().svk_gated_ffn_bwd_workspace(dt, px, ldx, pw, ldw, M, H, K, int(dw), int(db)) if M else 0
+        ws = _bytes(nb, x)
+        if M:
+            _on(x, "svk_gated_ffn_bwd", dt, px, ldx, pw, ldw, pre.data_ptr(), dh.data_ptr(), lddh, _p(gx), K, _p(gw),
+                _p(gb), M, H, K, code, _p(ws), nb)
+        else:
+            for t in (gw, gb):
+                if t is not None:
+                    t.zero_()
+    return gx, gw, gb
+
+
+def quant_rows(x):
+    """(codes int8 [..., K], scale float32 [...]) with x ~ codes * scale: scale = max |row| / 127, codes rounded to the
+    nearest, ties to even (svk_quant_rows).  Tokens before ``gemm_i8``; a weight [N, K] once, when it is loaded.  Rows of
+    the codes are 16 bytes apart at least (a view of a padded buffer where K % 16 != 0)."""
+    fn = "quant_rows"
+    dt = dtype_code(x.dtype)
+    _chk(x, "x")
+    M, K, ldx = _token_rows(x, fn, "x")
+    ldq = (K + 15) // 16 * 16
+    lead = x.shape[:-1]
+    q = torch.empty(*lead, ldq, device=x.device, dtype=torch.int8)
+    s = torch.empty(lead, device=x.device, dtype=torch.float32)
+    if M:
+        _on(x, "svk_quant_rows", dt, x.data_ptr(), ldx, q.data_ptr(), ldq, s.data_ptr(), M, K)
+    return (q if ldq == K else q[..., :K]), s
+
+
+def gemm_i8(a, a_scale, w, w_scale, bias=None, act=None, residual=None, out=None, dtype=torch.float16):
+    """act((a @ w.T as exact integers) * a_scale[m] * w_scale[n] + bias) + residual (svk_gemm_i8): a int8 [..., K] with
+    a_scale float32 [...], w int8 [N, K] with w_scale float32 [N] (both from quant_rows) -> [..., N] in ``dtype`` (or
+    out's).  K <= 131072.  ``out`` may be ``residual``."""
+    fn = "gemm_i8"
+    _chk(a, "a", torch.int8); _chk(w, "w", torch.int8)
+    M, K, lda = _token_rows(a, fn, "a")
+    if w.dim() != 2 or w.shape[1] != K or w.shape[0] == 0:
+        raise _lib.SvkError(f"svk.{fn}: w {tuple(w.shape)} does not match K={K}")
+    _, _, ldw = _token_rows(w, fn, "w")
+    N = w.shape[0]
+    _vector(a_scale, M, fn, "a_scale"); _vector(w_scale, N, fn, "w_scale"); _vector(bias, N, fn, "bias")
+    lead = a.shape[:-1]
+    if out is None:
+        out, ldy = torch.empty(*lead, N, device=a.device, dtype=dtype), N
+    else:
+        _chk(out, "out")
+        if out.shape != (*lead, N):
+            raise _lib.SvkError(f"svk.{fn}: out is {tuple(out.shape)}, not {(*lead, N)}")
+        _, _, ldy = _token_rows(out, fn, "out")
+        if not (_apart(out, a) and _apart(out, w) and _apart(out, residual)):
+            raise _lib.SvkError(f"svk.{fn}: out overlaps an input")
+    dt = dtype_code(out.dtype)
+    ldr = 0
+    if residual is not None:
+        _chk(residual, "residual", out.dtype)
+        if residual.shape != out.shape:
+            raise _lib.SvkError(f"svk.{fn}: residual is {tuple(residual.shape)}, not {tuple(out.shape)}")
+        _, _, ldr = _token_rows(residual, fn, "residual")
+    if act not in ACT:
+        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(k for k in ACT if k)}")
+    _same_device(fn, a, a_scale, w, w_scale, bias, residual, out)
+    if M:
+        pa, pw = a.data_ptr(), w.data_ptr()
+        nb = _lib.load().svk_gemm_i8_workspace(pa, lda, pw, ldw, M, N, K)
+        ws = _bytes(nb, a)
+        _on(a, "svk_gemm_i8", dt, pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), _p(bias), _p(residual), ldr,
+            out.data_ptr(), ldy, M, N, K, ACT[act], _p(ws), nb)
+    return out

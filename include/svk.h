@@ -32,6 +32,8 @@ extern "C" {
 
 enum { SVK_F32 = 0, SVK_BF16 = 1, SVK_F16 = 2 };
 enum { SVK_ACT_NONE = 0, SVK_ACT_GELU = 1, SVK_ACT_RELU = 2, SVK_ACT_TANH = 3 };
+enum { SVK_GLU_SILU = 0, SVK_GLU_GELU = 1, SVK_GLU_RELU = 2 };      /* activation of svk_gated_ffn's gate */
+enum { SVK_POS_I32 = 0, SVK_POS_I64 = 1, SVK_POS_F32 = 2 };          /* type of svk_rope3d's positions */
 enum { SVK_OK = 0, SVK_EINVAL = -1, SVK_EUNSUPPORTED = -2, SVK_ELAUNCH = -3 };
 
 const char* svk_version(void);
@@ -588,6 +590,48 @@ int svk_pack_params8(int dtype, const void* desc, int ndesc, long total, const f
  * master matrix): tiles of 64 x 64 through LDS so both the master reads and the packed writes are
  * coalesced.  tiles: device array of ntiles {long src, dst; int K, N, n0, k0} (one per tile). */
 int svk_pack_transpose(int dtype, const void* tiles, int ntiles, const float* src, void* dst, void* stream);
+
+/* Rotary positions with three axes (csrc/rope3d.hip), applied to q and k before svk_attention: tokens of a video lie at
+ * (time, row, column).  Pair i of every head (R = nt + nh + nw pairs: the first nt follow time, then nh rows, nw columns)
+ * is turned by th = pos[axis(i)] * freqs[i]: (x, y) -> (x cos th - y sin th, x sin th + y cos th); inverse != 0 turns by
+ * -th, which is the gradient.  Pairs are channels (i, i + R) of a head, or (2i, 2i + 1) if interleaved; channels 2R ..
+ * hd - 1 are copied.  Q / K [B, N, heads * hd] with unit channel stride, ld* values between tokens and sb* between
+ * batches; kv_heads = 0: no K.  pos [B, N, 3] of pos_type (SVK_POS_*), unit stride in the last dim, sbp = 0: the same
+ * positions for every batch.  freqs [R] f64, radians a step.  Outputs may be the inputs themselves (same strides).
+ * Angles are formed in 64 bits; a position that is not finite gives NaN in the channels that follow its axis. */
+int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo, long ldqo, long sbqo, int heads, const void* K,
+               long ldk, long sbk, void* Ko, long ldko, long sbko, int kv_heads, const void* pos, int pos_type, long ldp,
+               long sbp, const double* freqs, int nt, int nh, int nw, int hd, int B, int N, int interleaved, int inverse,
+               void* stream);
+
+/* Gated feed-forward block (csrc/gated_ffn.hip): Hout = act(X Wg^T + bg) * (X Wu^T + bu), one kernel.  X [M, K], W =
+ * [Wg; Wu] [2H, K], bias = [bg; bu] [2H] f32 or NULL, Hout [M, H]; act = SVK_GLU_*.  pre (NULL, or [M, 2H] contiguous):
+ * receives the two projections rounded to dtype, for svk_gated_ffn_bwd.  ws: svk_gated_ffn_workspace bytes (0 where the
+ * rows of X and W are whole 16-byte pieces; 16-byte aligned otherwise). */
+long svk_gated_ffn_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K);
+int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, long ldw, const float* bias, void* Hout, long ldh,
+                  void* pre, long M, long H, long K, int act, void* ws, long ws_bytes, void* stream);
+/* Its backward pass from dH [M, H] and pre: with dP = [dH * u * act'(g) | dH * act(g)] (rounded to dtype once)
+ * dX [M, K] = dP W, dW [2H, K] contiguous = dP^T X, db [2H] f32 = column sums of dP before its rounding.  Each of dX, dW,
+ * db may be NULL; they are written, not added to, in the same order of summation on every run.  ws:
+ * svk_gated_ffn_bwd_workspace bytes, 16-byte aligned. */
+long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K,
+                                 int want_dw, int want_db);
+int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH,
+                      long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K, int act, void* ws,
+                      long ws_bytes, void* stream);
+
+/* 8-bit integer products (csrc/gemm_i8.hip).  svk_quant_rows: S[m] = max |X[m, :]| / 127, Q[m, k] = X[m, k] / S[m] rounded
+ * to the nearest integer (ties to even); a row of zeros has S = 0 and codes 0, a row with an infinity or a NaN S = NaN
+ * and codes 0.  For weights [N, K] the same gives the scale of each output channel.
+ * svk_gemm_i8: Y = act((A W^T as integers) * sa[m] * sw[n] + bias[n]) + R, A [M, K] and W [N, K] int8, sa [M], sw [N],
+ * bias [N] f32 (or NULL), R (or NULL) and Y [M, N] in dtype.  The integer sums are exact: K <= 131072.  ws:
+ * svk_gemm_i8_workspace bytes (0 where the rows of A and W are whole 16-byte pieces; 16-byte aligned otherwise). */
+int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long ldq, float* S, long M, long K, void* stream);
+long svk_gemm_i8_workspace(const void* A, long lda, const void* W, long ldw, long M, long N, long K);
+int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, const void* W, long ldw, const float* sw,
+                const float* bias, const void* R, long ldr, void* Y, long ldy, long M, long N, long K, int act, void* ws,
+                long ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,171 @@
+"""Host logic of the token-block operators (rope3d, gated_ffn, quant_rows / gemm_i8) without a GPU: argument checks of
+the C ABI (made before any launch, so the made-up addresses are never read), workspace sizes, rotary frequencies, and
+the views the wrappers accept as rows or as outputs."""
+import math
+
+import pytest
+import torch
+
+A = 0x10000          # a made-up, 16-byte aligned device address
+
+
+def _lib():
+    from svk import _lib as L
+    return L.load()
+
+
+def _rope(lib, **kw):
+    a = dict(dt=0, q=A, qo=A, heads=2, k=A, ko=A, kv=1, pos=A, pt=0, freqs=A, nt=2, nh=1, nw=1, hd=8, B=1, N=4, il=0)
+    a.update(kw)
+    return lib.svk_rope3d(a["dt"], a["q"], 16, 64, a["qo"], 16, 64, a["heads"], a["k"], 8, 32, a["ko"], 8, 32, a["kv"],
+                          a["pos"], a["pt"], 3, 0, a["freqs"], a["nt"], a["nh"], a["nw"], a["hd"], a["B"], a["N"],
+                          a["il"], 0, None)
+
+
+@pytest.mark.parametrize("kw", [dict(q=None), dict(qo=None), dict(heads=0), dict(k=None), dict(ko=None), dict(kv=-1),
+                                dict(pos=None), dict(freqs=None), dict(nt=-1), dict(nt=0, nh=0, nw=0), dict(nt=3),
+                                dict(pt=3), dict(B=-1), dict(N=-1), dict(dt=7)])
+def test_rope3d_refuses(kw):
+    lib = _lib()
+    assert _rope(lib, **kw) == -1 and lib.svk_last_error()
+
+
+def test_rope3d_unsupported_and_empty():
+    lib = _lib()
+    assert _rope(lib, hd=4098) == -2 and b"head width" in lib.svk_last_error()
+    assert _rope(lib, hd=9, il=1) == -2 and b"interleaved" in lib.svk_last_error()
+    assert _rope(lib, B=65536, N=65536) == -2
+    assert _rope(lib, B=0) == 0 and _rope(lib, N=0) == 0          # nothing to launch
+
+
+def _gated(lib, **kw):
+    a = dict(dt=1, x=A, ldx=64, w=A, ldw=64, h=A, ldh=32, M=100, H=32, K=64, act=0, ws=None, n=0)
+    a.update(kw)
+    return lib.svk_gated_ffn(a["dt"], a["x"], a["ldx"], a["w"], a["ldw"], None, a["h"], a["ldh"], None, a["M"], a["H"],
+                             a["K"], a["act"], a["ws"], a["n"], None)
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(w=None), dict(h=None), dict(ldx=63), dict(ldw=63), dict(ldh=31),
+                                dict(M=-1), dict(H=0), dict(K=0), dict(act=3), dict(act=-1), dict(dt=5),
+                                dict(K=63, ldx=63, ldw=63)])         # the last: no workspace for the padded rows
+def test_gated_ffn_refuses(kw):
+    lib = _lib()
+    assert _gated(lib, **kw) == -1 and b"svk_gated_ffn" in lib.svk_last_error()
+
+
+def test_gated_ffn_sizes():
+    lib = _lib()
+    assert _gated(lib, M=0) == 0
+    assert _gated(lib, H=1 << 20, ldh=1 << 20, K=2048, ldx=2048, ldw=2048) == -2      # 8 GiB of weights
+    ws = lib.svk_gated_ffn_workspace
+    assert ws(1, A, 64, A, 64, 100, 32, 64) == 0
+    assert ws(1, A, 63, A, 63, 100, 32, 63) == (100 + 64) * 128      # both padded to 128-byte rows
+    assert ws(1, A + 2, 64, A, 64, 100, 32, 64) == 100 * 128         # x misaligned
+    assert ws(1, A, 63, A, 63, 8, 32, 63) == 0                       # few tokens: read as they are
+
+
+def _gated_bwd(lib, **kw):
+    a = dict(dt=0, x=A, w=A, pre=A, dh=A, lddh=32, dx=A, lddx=64, dw=A, db=A, M=100, H=32, K=64, act=0, ws=A, n=1 << 30)
+    a.update(kw)
+    return lib.svk_gated_ffn_bwd(a["dt"], a["x"], 64, a["w"], 64, a["pre"], a["dh"], a["lddh"], a["dx"], a["lddx"], a["dw"],
+                                 a["db"], a["M"], a["H"], a["K"], a["act"], a["ws"], a["n"], None)
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(w=None), dict(pre=None), dict(dh=None), dict(lddh=31), dict(lddx=63),
+                                dict(M=-1), dict(H=0), dict(K=0), dict(act=9), dict(dt=3), dict(ws=None), dict(ws=A + 8),
+                                dict(n=100)])
+def test_gated_ffn_bwd_refuses(kw):
+    lib = _lib()
+    assert _gated_bwd(lib, **kw) == -1 and b"svk_gated_ffn_bwd" in lib.svk_last_error()
+
+
+def test_gated_ffn_bwd_workspace_covers_its_parts():
+    lib = _lib()
+    for es, dt in ((2, 1), (2, 2), (4, 0)):
+        for M, H, K in ((1, 1, 1), (100, 33, 64), (5000, 96, 61), (20000, 40, 72)):
+            ld = (2 * H * es + 15) // 16 * 16
+            full = lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 1, 1)
+            assert full >= M * ld + math.ceil(M / 64) * 2 * H * 4
+            assert lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 0, 0) <= full
+    assert lib.svk_gated_ffn_bwd_workspace(1, A, 8, A, 8, 0, 8, 8, 1, 1) == 0
+
+
+def _i8(lib, **kw):
+    a = dict(dt=2, a=A, lda=64, sa=A, w=A, ldw=64, sw=A, R=None, ldr=0, y=A, ldy=48, M=100, N=48, K=64, act=0, ws=None, n=0)
+    a.update(kw)
+    return lib.svk_gemm_i8(a["dt"], a["a"], a["lda"], a["sa"], a["w"], a["ldw"], a["sw"], None, a["R"], a["ldr"], a["y"],
+                           a["ldy"], a["M"], a["N"], a["K"], a["act"], a["ws"], a["n"], None)
+
+
+@pytest.mark.parametrize("kw", [dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None), dict(lda=63),
+                                dict(ldw=63), dict(ldy=47), dict(R=A, ldr=47), dict(M=-1), dict(N=0), dict(K=0),
+                                dict(K=131073, lda=131073, ldw=131073), dict(act=4), dict(act=-1),
+                                dict(lda=65)])                        # the last: rows to be padded, no workspace
+def test_gemm_i8_refuses(kw):
+    lib = _lib()
+    assert _i8(lib, **kw) == -1 and b"svk_gemm_i8" in lib.svk_last_error()
+
+
+def test_gemm_i8_and_quant_rows_sizes():
+    lib = _lib()
+    assert _i8(lib, M=0) == 0
+    assert _i8(lib, dt=9, M=8) == -1
+    assert _i8(lib, N=1 << 20, ldy=1 << 20, K=8192, lda=8192, ldw=8192) == -2
+    assert lib.svk_gemm_i8_workspace(A, 61, A, 61, 100, 48, 61) == 148 * 64
+    assert lib.svk_gemm_i8_workspace(A, 64, A, 61, 100, 48, 61) == 148 * 64
+    assert lib.svk_quant_rows(0, A, 8, A, 8, A, 0, 8, None) == 0
+    for bad in ((0, None, 8, A, 8, A, 1, 8), (0, A, 7, A, 8, A, 1, 8), (0, A, 8, A, 7, A, 1, 8), (0, A, 8, A, 8, A, -1, 8),
+                (0, A, 8, A, 8, A, 1, 0), (0, A, 8, None, 8, A, 1, 8), (0, A, 8, A, 8, None, 1, 8), (8, A, 8, A, 8, A, 1, 8)):
+        assert lib.svk_quant_rows(*bad, None) == -1
+
+
+def test_rope3d_freqs():
+    import svk
+    from svk import ops
+    f = ops.rope3d_freqs((4, 2, 0), base=100.0, device="cpu")
+    assert f.dtype == torch.float64
+    assert f.tolist() == pytest.approx([1, 100 ** -0.25, 100 ** -0.5, 100 ** -0.75, 1, 100 ** -0.5], rel=1e-15)
+    f = ops.rope3d_freqs((2, 1, 1), base=16.0, shared=True, device="cpu")
+    assert f.tolist() == pytest.approx([1, 0.5, 0.25, 0.125], rel=1e-15)
+    for bad in ((0, 0, 0), (1, 2), (-1, 2, 2)):
+        with pytest.raises(svk.SvkError, match="sections"):
+            ops.rope3d_freqs(bad, device="cpu")
+
+
+def test_no_cpu_path():
+    import svk
+    from svk import ops
+    x = torch.zeros(4, 8)
+    for call in (lambda: ops.rope3d(x[None], None, torch.zeros(4, 3), torch.ones(3, dtype=torch.float64), (1, 1, 1), 1),
+                 lambda: ops.gated_ffn(x, x), lambda: ops.gated_ffn_bwd(x, x, x, x), lambda: ops.quant_rows(x),
+                 lambda: ops.gemm_i8(x.char(), x[:, 0], x.char(), x[:, 0])):
+        with pytest.raises(svk.SvkError, match="GPU"):
+            call()
+
+
+def test_token_rows_views():
+    import svk
+    from svk import ops
+    rows = lambda t: ops._token_rows(t, "f", "x")  # noqa: E731
+    b = torch.zeros(5, 7, 24)
+    assert rows(b) == (35, 24, 24)
+    assert rows(b[:, :, 8:16]) == (35, 8, 24)
+    assert rows(b[:, -1:]) == (5, 24, 7 * 24)          # the newest token of every batch
+    assert rows(b[2, 3]) == (1, 24, 24)
+    assert rows(b[:, 3, :8]) == (5, 8, 7 * 24)
+    assert rows(b[:1, :1]) == (1, 24, 24)
+    assert rows(b[:0])[0] == 0
+    for bad in (b[:, :5], b.transpose(0, 1), b.transpose(1, 2), torch.zeros(3, 0), torch.zeros(1, 8).expand(4, 8)):
+        with pytest.raises(svk.SvkError):
+            rows(bad)
+
+
+def test_apart_views():
+    from svk import ops
+    b = torch.zeros(4, 6, 30)
+    q, k, v = b[..., :10], b[..., 10:20], b[..., 20:]
+    assert ops._apart(q, k) and ops._apart(v, q) and ops._apart(q, q) and ops._apart(q, torch.zeros(4, 6, 10))
+    assert ops._apart(b[:2], b[2:]) and ops._apart(q, None) and ops._apart(b[:0], b)
+    assert not ops._apart(q, b[..., 5:15]) and not ops._apart(b[..., 5:15], q)
+    assert not ops._apart(b[:3], b[1:]) and not ops._apart(b[..., 25:], b.flatten()[5:])
+    assert not ops._apart(q, b.view(torch.float16)[..., :10])
