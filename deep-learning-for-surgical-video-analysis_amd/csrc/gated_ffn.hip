@@ -52,32 +52,22 @@ __device__ __forceinline__ void glu_grad(float g, int act, float& a, float& d) {
   }
 }
 
-// 4 consecutive values of a row as one store (V4), or those that exist one by one
-template <typename T>
-__device__ __forceinline__ void put4(T* at, const float* v, int n, bool v4) {
-  T o[4] = {from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};
-  if (v4 && n >= 4) {
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(o);
-    else *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(o);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) at[e] = o[e];
-  }
-}
-
-template <typename T>
+// ACT: the activation, or -1: `act`, chosen while running (few tokens)
+template <typename T, int ACT>
 struct GateEpi {
   T* h; long ldh;
   T* pre;                 // [M, 2H] contiguous, or null
   const float* bias;      // [2H] or null
   int M, H, act;
-  bool v4, p4;            // 4-value stores of h / of pre are aligned
 
-  template <class C> __device__ __forceinline__ int row(int r, int tn) const {
-    const int w = r / C::WN, in = r % C::WN, up = in >= C::WN / 2;
-    const int c = tn * (C::BN / 2) + w * (C::WN / 2) + in - up * (C::WN / 2);
-    return min(c, H - 1) + up * H;
+  __device__ __forceinline__ float activate(float g) const { return glu_act<T>(g, ACT < 0 ? act : ACT); }
+  // a wave's columns: half gate, half up rows of the same hidden channels; the pairs of blocks interleaved where each
+  // half has two
+  template <class C> static constexpr int width() { return C::TN >= 4 ? 8 : 4; }
+  template <class C> __device__ __forceinline__ long first(int tn) const { return (long)tn * (C::BN / 2); }
+  template <class C> __device__ __forceinline__ uint32_t offset(int r, uint32_t ldb) const {
+    const int in = r % C::WN, up = in >= C::WN / 2, c = in - up * (C::WN / 2);
+    return (uint32_t)(r / C::WN * (C::WN / 2) + (width<C>() == 8 ? pair_col(c) : c) + up * H) * ldb;
   }
   __device__ __forceinline__ int skinny_row(int bid, int j, int fr) const { return min(bid * 16 + fr, H - 1) + j * H; }
   __device__ __forceinline__ void skinny_write(int bid, int m, int n, float g, float u) const {
@@ -91,55 +81,52 @@ struct GateEpi {
       pre[(long)m * 2 * H + c] = from_f<T>(g);
       pre[(long)m * 2 * H + H + c] = from_f<T>(u);
     }
-    h[(long)m * ldh + c] = from_f<T>(glu_act<T>(g, act) * u);
+    h[(long)m * ldh + c] = from_f<T>(activate(g) * u);
   }
   template <class C, typename A>
-  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
-    constexpr int TG = C::TN / 2;
-    static_assert(C::TN % 2 == 0, "a wave's columns are half gate, half up");
+  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int) const {
+    constexpr int TG = C::TN / 2, W = width<C>(), S = W / 4;
+    static_assert(C::TN % 2 == 0 && TG % S == 0, "a wave's columns are half gate, half up");
 #pragma unroll
-    for (int j = 0; j < TG; ++j) {
-      const int c = tn * (C::BN / 2) + wn * (C::WN / 2) + j * 16 + fq * 4, left = H - c;
+    for (int j = 0; j < TG; j += S) {
+      const int c = tn * (C::BN / 2) + wn * (C::WN / 2) + j * 16 + fq * W, left = H - c;
       if (left <= 0) continue;
-      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
-      if (bias)
+      float bg[W], bu[W];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < left) {
-            bg[e] = bias[c + e];
-            bu[e] = bias[H + c + e];
-          }
+      for (int e = 0; e < W; ++e) {
+        const int at = min(c + e, H - 1);
+        bg[e] = bias ? bias[at] : 0.f;
+        bu[e] = bias ? bias[H + at] : 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) {
         const int m = m0 + i * 16;
         if (m >= M) continue;
-        float g[4], u[4], o[4];
+        float g[W], u[W], o[W];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = acc[i][j][e] + bg[e];
-          u[e] = acc[i][j + TG][e] + bu[e];
-          o[e] = glu_act<T>(g[e], act) * u[e];
+        for (int e = 0; e < W; ++e) {
+          g[e] = acc[i][j + e / 4][e % 4] + bg[e];
+          u[e] = acc[i][j + TG + e / 4][e % 4] + bu[e];
+          o[e] = activate(g[e]) * u[e];
         }
         if (pre) {
-          put4<T>(pre + (long)m * 2 * H + c, g, left, p4);
-          put4<T>(pre + (long)m * 2 * H + H + c, u, left, p4);
+          put<T, W, C::NONTEMPORAL>(pre + (long)m * 2 * H + c, g, left);
+          put<T, W, C::NONTEMPORAL>(pre + (long)m * 2 * H + H + c, u, left);
         }
-        put4<T>(h + (long)m * ldh + c, o, left, v4);
+        put<T, W, C::NONTEMPORAL>(h + (long)m * ldh + c, o, left);
       }
     }
   }
 };
 
-// plain product: rounded to T, or an f32 slab of one part of the reduction
+// plain product of a col operand B: rounded to T, or an f32 slab of one part of the reduction
 template <typename T>
 struct PlainEpi {
   T* y; long ldy;
   float* slab;            // [parts][M][N], or null
   int M, N;
-  bool v4, s4;
-  template <class C> __device__ __forceinline__ int row(int r, int tn) const { return min(tn * C::BN + r, N - 1); }
   template <class C, typename A>
-  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
+  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int part) const {
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
       const int n = tn * C::BN + wn * C::WN + j * 16 + fq * 4, left = N - n;
@@ -149,8 +136,8 @@ struct PlainEpi {
         const int m = m0 + i * 16;
         if (m >= M) continue;
         const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (slab) put4<float>(slab + ((long)blockIdx.y * M + m) * N + n, v, left, s4);
-        else put4<T>(y + (long)m * ldy + n, v, left, v4);
+        if (slab) put<float, 4, false>(slab + ((long)part * M + m) * N + n, v, left);
+        else put<T, 4, C::NONTEMPORAL>(y + (long)m * ldy + n, v, left);
       }
     }
   }
@@ -247,21 +234,12 @@ inline int pick(long m, long n, long parts = 1) {
   return 2;
 }
 
-template <typename T, class C, bool AC, bool BC, class Epi>
-static int go(Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
-  p.ntm = (int)((m + C::BM - 1) / C::BM);
-  p.ntn = (int)((n + C::BN - 1) / C::BN);
-  if ((long)p.ntm * p.ntn > 0x7fffffffL) { set_error("%s: too many tiles", name); return SVK_EUNSUPPORTED; }
-  hipLaunchKernelGGL((tile_mm<T, C, AC, BC, Epi>), dim3(p.ntm * p.ntn, p.parts), dim3(C::NT), 0, st, p, epi);
-  set_last_kernel(name);
-  return check_launch(name);
-}
 template <typename T, bool AC, bool BC, class Epi>
 static int tiled(int cfg, Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
   p.nk = (p.K + 128 / (int)sizeof(T) - 1) / (128 / (int)sizeof(T));
-  if (cfg == 0) return go<T, Big, AC, BC>(p, m, n, epi, st, name);
-  if (cfg == 1) return go<T, Mid, AC, BC>(p, m, n, epi, st, name);
-  return go<T, Small, AC, BC>(p, m, n, epi, st, name);
+  if (cfg == 0) return launch_tiles<T, Big, AC, BC>(p, m, n, epi, st, name);
+  if (cfg == 1) return launch_tiles<T, Mid, AC, BC>(p, m, n, epi, st, name);
+  return launch_tiles<T, Small, AC, BC>(p, m, n, epi, st, name);
 }
 
 template <typename T, int MT, class Epi>
@@ -271,8 +249,6 @@ static int skinny_mt(const Args& p, bool vec, int blocks, const Epi& epi, hipStr
   set_last_kernel("skinny_mm");
   return check_launch("skinny_mm");
 }
-
-constexpr int SKINNY_M = 32;
 
 // the weight gradient's split of the token axis: small outputs would leave most CUs idle over a long reduction
 inline int dw_parts(long n2, long k, long m, int bk) {
@@ -349,13 +325,11 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
-    GateEpi<T> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, false, false};
-    epi.v4 = H % 4 == 0 && ldh % 4 == 0 && ((uintptr_t)Hout & (4 * es - 1)) == 0;
-    epi.p4 = H % 4 == 0 && ((uintptr_t)pre & (4 * es - 1)) == 0;
-    Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, (int)M, (int)(2 * H), (int)K, 0, 0, 0, 1};
+    Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(X, ldx, K, es) && rows_ok(W, ldw, K, es);
       const int blocks = (int)((H + 15) / 16);
+      GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act};
       return M <= 16 ? skinny_mt<T, 1>(p, vec, blocks, epi, st) : skinny_mt<T, 2>(p, vec, blocks, epi, st);
     }
     char* at = (char*)ws;
@@ -372,7 +346,15 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
       p.ldb = ldk;
       p.K = (int)(ldk / es);
     }
-    return tiled<T, false, false>(pick(M, 2 * H), p, M, 2 * H, epi, st, "gated_ffn");
+    p.abytes = (M - 1) * p.lda + p.K * es;
+    p.bbytes = (2 * H - 1) * p.ldb + p.K * es;
+    auto run = [&](auto act_c) {
+      GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act};
+      return tiled<T, false, false>(pick(M, 2 * H), p, M, 2 * H, epi, st, "gated_ffn");
+    };
+    if (act == SVK_GLU_SILU) return run(std::integral_constant<int, SVK_GLU_SILU>{});
+    if (act == SVK_GLU_GELU) return run(std::integral_constant<int, SVK_GLU_GELU>{});
+    return run(std::integral_constant<int, SVK_GLU_RELU>{});
   });
 }
 
@@ -418,13 +400,13 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     char* at = (char*)ws;
     T* D = (T*)at;
     at += need.dpre;
-    Args px{(const char*)X, nullptr, ldx * es, 0, 0, 0, 0, 0, 0, 0, 1};
-    const char* Wr = (const char*)W;
-    long ldwb = ldw * es;
+    const char *Xr = (const char*)X, *Wr = (const char*)W;
+    long ldxb = ldx * es, ldwb = ldw * es;
+    const long kb = padx ? ldk : K * es;            // bytes of a row of either
     if (padx) {
       if (int rc = pad<T>(X, ldx, at, M, K, st)) return rc;
-      px.A = at;
-      px.lda = ldk;
+      Xr = at;
+      ldxb = ldk;
       at += need.x;
       if (int rc = pad<T>(W, ldw, at, 2 * H, K, st)) return rc;
       Wr = at;
@@ -450,17 +432,14 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
       if (int rc = check_launch("join_bias")) return rc;
     }
     if (dX) {
-      PlainEpi<T> epi{(T*)dX, lddx, nullptr, (int)M, (int)K, false, false};
-      epi.v4 = lddx % 4 == 0 && ((uintptr_t)dX & (4 * es - 1)) == 0;
+      PlainEpi<T> epi{(T*)dX, lddx, nullptr, (int)M, (int)K};
       // the padding of D is zero and rows of W past 2H read as zero, so the reduction runs over whole chunks
-      Args p{(const char*)D, Wr, need.ldd * es, ldwb, (int)M, (int)K, (int)(2 * H), 0, 0, 0, 1};
+      Args p{(const char*)D, Wr, need.ldd * es, ldwb, M * need.ldd * es, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1};
       if (int rc = tiled<T, false, true>(pick(M, K), p, M, K, epi, st, "gated_ffn_dx")) return rc;
     }
     if (dW) {
-      PlainEpi<T> epi{(T*)dW, K, slabs, (int)(2 * H), (int)K, false, false};
-      epi.v4 = K % 4 == 0 && ((uintptr_t)dW & (4 * es - 1)) == 0;
-      epi.s4 = K % 4 == 0;
-      Args p{(const char*)D, px.A, need.ldd * es, px.lda, (int)(2 * H), (int)K, (int)M, 0, 0, 0, need.parts};
+      PlainEpi<T> epi{(T*)dW, K, slabs, (int)(2 * H), (int)K};
+      Args p{(const char*)D, Xr, need.ldd * es, ldxb, M * need.ldd * es, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, need.parts};
       const int cfg = need.parts > 1 ? 1 : pick(2 * H, K);
       if (int rc = tiled<T, true, true>(cfg, p, 2 * H, K, epi, st, "gated_ffn_dw")) return rc;
       if (slabs) {

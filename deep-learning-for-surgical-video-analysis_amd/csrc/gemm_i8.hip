@@ -88,20 +88,21 @@ __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long 
   }
 }
 
-template <typename T>
+// ACT: none, GELU, or -1: `act`, chosen while running
+template <typename T, int ACT>
 struct ScaleEpi {
   const float *sa, *sw, *bias;
   const T* R; long ldr;
   T* y; long ldy;
   int M, N, act;
-  bool v4;
 
   __device__ __forceinline__ float value(int acc, float a, float w, float b) const {
     const float v = (float)acc * a * w + b;
-    if constexpr (sizeof(T) == 4) return apply_act(v, act);
-    else return apply_act_fast(v, act);
+    if constexpr (sizeof(T) == 4) return apply_act(v, ACT < 0 ? act : ACT);
+    else return apply_act_fast(v, ACT < 0 ? act : ACT);
   }
-  template <class C> __device__ __forceinline__ int row(int r, int tn) const { return min(tn * C::BN + r, N - 1); }
+  template <class C> __device__ __forceinline__ long first(int tn) const { return (long)tn * C::BN; }
+  template <class C> __device__ __forceinline__ uint32_t offset(int r, uint32_t ldb) const { return (uint32_t)pair_col(r) * ldb; }
   __device__ __forceinline__ int skinny_row(int bid, int j, int fr) const { return min(bid * 32 + j * 16 + fr, N - 1); }
   __device__ __forceinline__ void skinny_write(int bid, int m, int n, int v0, int v1) const {
     one(m, bid * 32 + n, v0);
@@ -114,42 +115,59 @@ struct ScaleEpi {
     y[(long)m * ldy + n] = from_f<T>(v);
   }
   template <class C, typename A>
-  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
+  __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int) const {
+    constexpr int NW = 8 * sizeof(T) / 4;
+    typedef uint32_t vec __attribute__((ext_vector_type(NW)));
+    typedef vec anywhere __attribute__((aligned(2)));
+    float a[C::TM];
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) {
-      const int n = tn * C::BN + wn * C::WN + j * 16 + fq * 4, left = N - n;
+    for (int i = 0; i < C::TM; ++i) a[i] = sa[min(m0 + i * 16, M - 1)];
+#pragma unroll
+    for (int j = 0; j < C::TN; j += 2) {
+      const int n = tn * C::BN + wn * C::WN + j * 16 + fq * 8, left = N - n;
       if (left <= 0) continue;
-      float w[4], b[4];
+      float w[8], b[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const int c = min(n + e, N - 1);
         w[e] = sw[c];
         b[e] = bias ? bias[c] : 0.f;
       }
+      // the residual of the next rows is read before these rows are stored: read behind a store it would wait for that
+      // store (R may be Y itself: every value is read before it is written, by the same lane)
+      constexpr int RB = C::TM >= 4 ? 8 / (int)sizeof(T) : C::TM;  // rows in hand: 16 registers
+      vec r[2][RB];
+      auto fetch = [&](int i0, vec* o) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const int m = m0 + i * 16;
-        if (m >= M) continue;
-        const float a = sa[m];
-        T o[4];
-        typedef T vec __attribute__((ext_vector_type(4)));
-        vec r = {T(0), T(0), T(0), T(0)};
-        if (R) {
-          if (v4) r = *reinterpret_cast<const vec*>(R + (long)m * ldr + n);
-          else
-            for (int e = 0; e < 4; ++e)
-              if (e < left) r[e] = R[(long)m * ldr + n + e];
-        }
+        for (int i = 0; i < RB; ++i) {
+          const T* at = R + (long)min(m0 + (i0 + i) * 16, M - 1) * ldr + n;
+          if (left >= 8) o[i] = *reinterpret_cast<const anywhere*>(at);
+          else {
+            T t[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = value(acc[i][j][e], a, w[e], b[e]);
-          o[e] = from_f<T>(R ? v + to_f(r[e]) : v);
+            for (int e = 0; e < 8; ++e) t[e] = at[min(e, left - 1)];
+            __builtin_memcpy(&o[i], t, sizeof(vec));
+          }
         }
-        T* at = y + (long)m * ldy + n;
-        if (v4) *reinterpret_cast<vec*>(at) = *reinterpret_cast<const vec*>(o);
-        else
-          for (int e = 0; e < 4; ++e)
-            if (e < left) at[e] = o[e];
+      };
+      if (R) fetch(0, r[0]);
+#pragma unroll
+      for (int i0 = 0; i0 < C::TM; i0 += RB) {
+        if (R && i0 + RB < C::TM) fetch(i0 + RB, r[(i0 / RB + 1) & 1]);
+#pragma unroll
+        for (int i = i0; i < i0 + RB; ++i) {
+          const int m = m0 + i * 16;
+          float v[8];
+          T t[8];
+          if (R) __builtin_memcpy(t, &r[(i0 / RB) & 1][i - i0], sizeof(vec));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = value(acc[i][j + e / 4][e % 4], a[i], w[e], b[e]);
+            if (R) v[e] += to_f(t[e]);
+          }
+          if (m < M) put<T, 8, C::NONTEMPORAL>(y + (long)m * ldy + n, v, left);
+          __builtin_amdgcn_sched_barrier(0);                    // one row at a time: fewer registers
+        }
       }
     }
   }
@@ -158,22 +176,11 @@ struct ScaleEpi {
 using Big = Tile<256, 256, 2, 4, 2, 2>;
 using Mid = Tile<128, 128, 2, 2, 2, 2>;
 using Small = Tile<64, 64, 2, 2, 4, 2>;
-constexpr int SKINNY_M = 32;
-
-template <typename T, class C>
-static int go(Args p, const ScaleEpi<T>& epi, hipStream_t st) {
-  p.ntm = (p.M + C::BM - 1) / C::BM;
-  p.ntn = (p.N + C::BN - 1) / C::BN;
-  if ((long)p.ntm * p.ntn > 0x7fffffffL) { set_error("svk_gemm_i8: too many tiles"); return SVK_EUNSUPPORTED; }
-  hipLaunchKernelGGL((tile_mm<int8_t, C, false, false, ScaleEpi<T>>), dim3(p.ntm * p.ntn), dim3(C::NT), 0, st, p, epi);
-  set_last_kernel("gemm_i8");
-  return check_launch("gemm_i8");
-}
 template <typename T, int MT>
-static int go_skinny(const Args& p, bool vec, const ScaleEpi<T>& epi, hipStream_t st) {
-  const int blocks = (p.N + 31) / 32;
-  if (vec) hipLaunchKernelGGL((skinny_mm<int8_t, MT, true, ScaleEpi<T>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
-  else hipLaunchKernelGGL((skinny_mm<int8_t, MT, false, ScaleEpi<T>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
+static int go_skinny(const Args& p, bool vec, const ScaleEpi<T, -1>& epi, hipStream_t st) {
+  const int blocks = (epi.N + 31) / 32;
+  if (vec) hipLaunchKernelGGL((skinny_mm<int8_t, MT, true, ScaleEpi<T, -1>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
+  else hipLaunchKernelGGL((skinny_mm<int8_t, MT, false, ScaleEpi<T, -1>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
   set_last_kernel("gemm_i8_skinny");
   return check_launch("gemm_i8_skinny");
 }
@@ -231,12 +238,10 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
-    ScaleEpi<T> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, false};
-    const uintptr_t am = 4 * sizeof(T) - 1;
-    epi.v4 = N % 4 == 0 && ldy % 4 == 0 && ((uintptr_t)Y & am) == 0 && (!R || (ldr % 4 == 0 && ((uintptr_t)R & am) == 0));
-    Args p{(const char*)A, (const char*)W, lda, ldw, (int)M, (int)N, (int)K, 0, 0, 0, 1};
+    Args p{(const char*)A, (const char*)W, lda, ldw, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(A, lda, K) && rows_ok(W, ldw, K);
+      ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act};
       return M <= 16 ? go_skinny<T, 1>(p, vec, epi, st) : go_skinny<T, 2>(p, vec, epi, st);
     }
     char* at = (char*)ws;
@@ -259,9 +264,17 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
       p.K = (int)ldk;
     }
     p.nk = (p.K + 127) / 128;
+    p.abytes = (M - 1) * p.lda + p.K;
+    p.bbytes = (N - 1) * p.ldb + p.K;
     auto tiles = [&](long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
-    if (tiles(256) >= 200) return go<T, Big>(p, epi, st);
-    if (tiles(128) >= 200) return go<T, Mid>(p, epi, st);
-    return go<T, Small>(p, epi, st);
+    auto run = [&](auto act_c) {
+      ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act};
+      if (tiles(256) >= 200) return launch_tiles<int8_t, Big, false, false>(p, M, N, epi, st, "gemm_i8");
+      if (tiles(128) >= 200) return launch_tiles<int8_t, Mid, false, false>(p, M, N, epi, st, "gemm_i8");
+      return launch_tiles<int8_t, Small, false, false>(p, M, N, epi, st, "gemm_i8");
+    };
+    if (act == SVK_ACT_NONE) return run(std::integral_constant<int, SVK_ACT_NONE>{});
+    if (act == SVK_ACT_GELU) return run(std::integral_constant<int, SVK_ACT_GELU>{});
+    return run(std::integral_constant<int, -1>{});
   });
 }

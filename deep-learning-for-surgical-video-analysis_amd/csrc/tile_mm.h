@@ -9,12 +9,23 @@
 //   lane's chunk in step s (A and B agree on which k that is, so the sum is the same set of products).
 // Col operands: 16-bit tiles are read back transposed by ds_read_b64_tr_b16 (as in wgrad_pk.hip), f32 by ds_read_b32.
 //
-// Staging: LDS-DMA (global_load_lds_dwordx4) into a ring of NS stages, one barrier a stage: a wave waits for its own
-// DMA of stage t, the barrier makes everyone's visible and ends the reads of stage t - 1, whose slot is then filled
-// with stage t + NS - 1 while stage t is multiplied.  16-byte chunks are XOR-swizzled on the source address so that
-// fragment reads are free of bank conflicts.
+// Staging: LDS-DMA (buffer_load ... lds, 16 bytes a lane) into a ring of NS stages.  A stage is two MFMA steps of 64
+// bytes of k; the fragments of one step are read while the other's are multiplied, so the LDS reads run under the MFMAs.
+// The stage's one barrier stands between its two steps: by then every wave holds the second step's fragments in
+// registers and its own DMA of the next stage has landed, so behind it the next stage can be read and this stage's slot
+// filled again.  That DMA is dealt between the MFMAs of the second step (issued in one go it held the wave's MFMAs up:
+// 16384 x 11264 x 2048 in bf16 went from 755 to 707 us with the persistent form below).
+// The lane offsets of the DMA are the same for every tile and stage; a tile or a stage is a descriptor's base, and its
+// range check gives zeros for rows past the end, so there is no branch and no address arithmetic in the loop.
 //
-// The MFMA is issued as B x A: a lane holds 4 consecutive n of one m, which the epilogue stores as one piece.
+// Persistent: the grid walks a stream of (tile, stage) and the DMA runs NS stages ahead of the products across tile
+// ends, so a tile's first stages are there when the last tile's results are written.  Results of the 256 x 256 tiles
+// are stored past the L2 (they are larger than it, and evicted the operands: 664 -> 631 us at the size above).
+// What is left (618 us, 1223 TFLOP/s; 1336 at 8192^3, where a plain library product reaches 1442): every CU writes its
+// tile at the same time, about 6 us a tile that nothing covers.
+//
+// The MFMA is issued as B x A: a lane holds 4 consecutive n of one m; pairs of 16-column blocks of a row operand B are
+// interleaved by fours, so that two blocks hold 8 consecutive n, one 16-byte store of a 16-bit type.
 #pragma once
 #include "svk_common.h"
 #include <type_traits>
@@ -27,22 +38,24 @@ typedef __attribute__((address_space(3))) void* las_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-static __device__ __attribute__((aligned(16))) uint4 g_zero[4];   // what a chunk past the end of K reads
+constexpr uint32_t OUTSIDE = 0xFFFFFFF0u;      // a lane offset past every descriptor's range: reads zeros
 
-// 16-byte LDS-DMA per lane: from sbase + voff (or a full address), to lds + 16 * lane
-__device__ __forceinline__ void dma16s(const char* sbase, uint32_t voff, uint32_t lds) {
-  const uint64_t b = reinterpret_cast<uint64_t>(sbase);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
-  sbase = reinterpret_cast<const char*>(((uint64_t)hi << 32) | (uint64_t)lo);
-  uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(voff), "s"(sbase), "s"(lds) : "memory");
+// buffer descriptor of the `left` bytes behind base (32-bit offsets; reads past them give zeros)
+__device__ __forceinline__ i32x4 descriptor(const char* base, long left) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint32_t n = left <= 0 ? 0u : (left > 0xFFFFFF00L ? 0xFFFFFF00u : (uint32_t)left);
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xFFFFu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)n);
+  r[3] = 0x00020000;                           // raw 32-bit data
+  return r;
 }
-__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+// 16 bytes a lane from the descriptor's base + voff to LDS lds + 16 * lane
+__device__ __forceinline__ void dma16(i32x4 r, uint32_t voff, uint32_t lds) {
   uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(voff), "s"(r), "s"(lds) : "memory");
 }
 
 template <typename T> struct Acc { typedef f32x4 t; };
@@ -66,11 +79,10 @@ __device__ __forceinline__ typename Acc<T>::t step(i32x4 b, i32x4 a, typename Ac
 struct Args {
   const char *A, *B;
   long lda, ldb;        // bytes between rows
-  int M, N;             // rows (row operands) or columns (col operands) of A and B that exist (row operand B: 32-bit
-                        // byte offsets, N * ldb < 2^32; A and col operands: 256 rows of 32-bit offsets a tile)
-  int K;                // reduction length in values; row operands: K * sizeof(T) % 16 == 0
+  long abytes, bbytes;  // bytes from A (B) to the end of its last row
+  int M, K;             // token rows (skinny_mm); reduction length in values
   int ntm, ntn;         // tiles
-  int nk, parts;        // stages in all; parts of the reduction (blockIdx.y), nk / parts stages each, rounded up
+  int nk, parts;        // stages of the reduction; parts it is split into, nk / parts stages each, rounded up, none empty
 };
 
 template <int BM_, int BN_, int WGM_, int WGN_, int NS_, int OCC_>
@@ -79,8 +91,9 @@ struct Tile {
   static constexpr int NT = 64 * WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int A_LD = A_BYTES / (NT * 16), B_LD = B_BYTES / (NT * 16), LD = A_LD + B_LD;
+  static constexpr bool NONTEMPORAL = BM >= 256;
   static_assert(A_BYTES % (NT * 16) == 0 && B_BYTES % (NT * 16) == 0, "whole DMA rounds");
-  static_assert(NS * STAGE <= 160 * 1024 && NS >= 2 && NS <= 4, "LDS ring");
+  static_assert(NS * STAGE <= 160 * 1024 && NS >= 2 && (NS - 1) * LD <= 63, "LDS ring, wait counter");
 };
 
 // chunk swizzle of row r of a col image of RB bytes a row: the 8 rows x 2 chunks of a 32-lane half of a transposed read
@@ -92,110 +105,123 @@ template <typename T, int RB> __device__ __forceinline__ int col_swz(int r) {
   else return ((r >> 2) & 3) << 2;
 }
 
-// XCD-aware tile order: workgroup ids are dealt round-robin to the 8 XCDs, so consecutive tiles go to one XCD's L2;
-// within it 8 row tiles are walked before the next column tile, for operand reuse
+// XCD-aware tile order: workgroups are dealt round-robin to the 8 XCDs, so consecutive tiles go to one XCD's L2; within
+// it 4 row tiles are walked before the next column tile, for operand reuse (2, 4, 8: within 1 %; 16: 3 % slower)
 __device__ __forceinline__ void tile_of(int bid, int ntm, int ntn, int& tm, int& tn) {
   const int n = ntm * ntn, xcd = bid & 7, q = n >> 3, r = n & 7;
   const int p = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
-  const int G = 8, per = G * ntn, grp = p / per, in = p - grp * per;
+  const int G = 4, per = G * ntn, grp = p / per, in = p - grp * per;
   const int g = min(G, ntm - grp * G);
   tm = grp * G + in % g;
   tn = in / g;
 }
 
-// Epi: static int row(int r, int tile): the B row of tile-local row r (row operands: which weight row it is);
-//      operator()(acc, m, n, ...) writes the tile
+// W consecutive values of a row: one store (of any alignment) where all W exist, else one by one
+template <typename T, int W, bool NTS>
+__device__ __forceinline__ void put(T* at, const float* v, int n) {
+  T o[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) o[e] = from_f<T>(v[e]);
+  typedef uint32_t vec __attribute__((ext_vector_type(W * sizeof(T) / 4)));
+  typedef vec anywhere __attribute__((aligned(2)));
+  if (n >= W) {
+    vec w;
+    __builtin_memcpy(&w, o, sizeof(w));
+    if constexpr (NTS) __builtin_nontemporal_store(w, reinterpret_cast<anywhere*>(at));
+    else *reinterpret_cast<anywhere*>(at) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (e < n) at[e] = o[e];
+  }
+}
+
+// position of tile-local B row r among the columns of its 32-column group: blocks of 16 interleaved by fours
+__device__ __forceinline__ int pair_col(int r) { return (r & ~31) + 8 * ((r >> 2) & 3) + 4 * ((r >> 4) & 1) + (r & 3); }
+
+// Epi (row operand B): uint32_t offset<C>(r, ldb): bytes from the tile's first row to B row r of the tile;
+//                      long first<C>(tn): the tile's first row
+//      write<C>(acc, m, tn, wn, fq, part): stores the tile; acc[i][j]: row m + 16 i, columns 4 fq .. of block j
 template <typename T, class C, bool ACOL, bool BCOL, class Epi>
 __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
   constexpr int ES = sizeof(T), BK = 128 / ES;
   constexpr int TM = C::TM, TN = C::TN, NS = C::NS;
   typedef typename Acc<T>::t acc_t;
-  static_assert(!(ACOL || BCOL) || ES >= 2, "col operands: 16 / 32-bit");
-  static_assert((C::BM * ES >= 128 && C::BN * ES >= 128) || !(ACOL || BCOL), "col images: rows of 8 chunks or more");
+  static_assert(!(ACOL || BCOL) || (ES >= 2 && C::BM * ES >= 128 && C::BN * ES >= 128), "col operands: 16 / 32-bit, rows of 8 chunks or more");
   __shared__ __attribute__((aligned(1024))) char smem[NS * C::STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / C::WGN, wn = wave % C::WGN;
   const int fr = lane & 15, fq = lane >> 4;
-  int tm, tn;
-  tile_of(blockIdx.x, p.ntm, p.ntn, tm, tn);
-  const int per = (p.nk + p.parts - 1) / p.parts;
-  const int k0 = blockIdx.y * per, k1 = min(k0 + per, p.nk);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(las_ptr)smem;
-
-  // DMA plan: instruction i of this wave fills 1 KiB = rows of the stage image.  Row operands: 8 rows of 128 bytes;
-  // col operands: 1024 / (tile bytes a row of k) rows of k.
   constexpr int ARB = ACOL ? C::BM * ES : 128, BRB = BCOL ? C::BN * ES : 128;      // image row bytes
-  uint32_t offA[C::A_LD], offB[C::B_LD];
-  const char* baseA = p.A + (ACOL ? (long)tm * C::BM * ES : (long)tm * C::BM * p.lda);
-  const char* baseB = p.B + (BCOL ? (long)tn * C::BN * ES : 0);
-  auto img = [&](int i, int rb, int& row, int& slot) {          // image row and chunk slot of this lane's 16 bytes
-    const int at = (wave + i * (C::NT / 64)) * 1024 + lane * 16;
-    row = at / rb;
-    slot = (at % rb) >> 4;
-  };
-#pragma unroll
-  for (int i = 0; i < C::A_LD; ++i) {
-    int r, s;
-    img(i, ARB, r, s);
-    if constexpr (ACOL) {
-      const int last = (p.M * ES - 1) / 16 - tm * (C::BM * ES / 16);   // last chunk of the row that exists
-      offA[i] = (uint32_t)r * (uint32_t)p.lda + min(s ^ col_swz<T, ARB>(r), last) * 16;
-    } else {
-      offA[i] = (uint32_t)min(r, p.M - 1 - tm * C::BM) * (uint32_t)p.lda + ((s ^ (r & 7)) << 4);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < C::B_LD; ++i) {
-    int r, s;
-    img(i, BRB, r, s);
-    if constexpr (BCOL) {
-      const int last = (p.N * ES - 1) / 16 - tn * (C::BN * ES / 16);
-      offB[i] = (uint32_t)r * (uint32_t)p.ldb + min(s ^ col_swz<T, BRB>(r), last) * 16;
-    } else {
-      offB[i] = (uint32_t)epi.template row<C>(r, tn) * (uint32_t)p.ldb + ((s ^ (r & 7)) << 4);   // by the epilogue's map
-    }
-  }
-  const char* zero = reinterpret_cast<const char*>(g_zero);
-  auto issue = [&](int kt) {
-    const uint32_t sa = lds0 + ((kt - k0) % NS) * C::STAGE, sb = sa + C::A_BYTES;
-    const bool tail = (kt + 1) * BK > p.K;
-#pragma unroll
-    for (int i = 0; i < C::A_LD; ++i) {
-      const uint32_t dst = sa + (wave + i * (C::NT / 64)) * 1024;
-      const char* src = baseA + (ACOL ? (long)kt * BK * p.lda : (long)kt * 128);
-      if (!tail) dma16s(src, offA[i], dst);
-      else {
-        int r, s;
-        img(i, ARB, r, s);
-        const int k = kt * BK + (ACOL ? r : (s ^ (r & 7)) * (16 / ES));
-        dma16(k < p.K ? src + offA[i] : zero, dst);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < C::B_LD; ++i) {
-      const uint32_t dst = sb + (wave + i * (C::NT / 64)) * 1024;
-      const char* src = baseB + (BCOL ? (long)kt * BK * p.ldb : (long)kt * 128);
-      if (!tail) dma16s(src, offB[i], dst);
-      else {
-        int r, s;
-        img(i, BRB, r, s);
-        const int k = kt * BK + (BCOL ? r : (s ^ (r & 7)) * (16 / ES));
-        dma16(k < p.K ? src + offB[i] : zero, dst);
-      }
-    }
-  };
+  const int units = p.ntm * p.ntn * p.parts, per = (p.nk + p.parts - 1) / p.parts;
+  if ((int)blockIdx.x >= units) return;
 
-  acc_t acc[TM][TN];
+  // DMA piece q of a stage: 1 KiB a wave of A's image, of B's from q = A_LD on
+  uint32_t offs[C::LD];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+  for (int q = 0; q < C::LD; ++q) {
+    const bool isA = q < C::A_LD;
+    const int rb = isA ? ARB : BRB, at = (wave + (isA ? q : q - C::A_LD) * (C::NT / 64)) * 1024 + lane * 16;
+    const int r = at / rb, s = (at % rb) >> 4;                  // image row, chunk slot
+    if (isA) offs[q] = (uint32_t)r * (uint32_t)p.lda + (ACOL ? s ^ col_swz<T, ARB>(r) : s ^ (r & 7)) * 16;
+    else if constexpr (BCOL) offs[q] = (uint32_t)r * (uint32_t)p.ldb + (s ^ col_swz<T, BRB>(r)) * 16;
+    else offs[q] = epi.template offset<C>(r, (uint32_t)p.ldb) + (s ^ (r & 7)) * 16;
+  }
+  const int kin = ((lane & 7) ^ (lane >> 3)) * (16 / ES);       // first k, within the stage, of a row operand's chunk
+
+  // the DMA's place in the stream: unit, stage, ring slot; its operand bases and the bytes behind them
+  int du = blockIdx.x, dkt = 0, dend = 0, dslot = 0;
+  const char *dA = nullptr, *dB = nullptr;
+  long lA = 0, lB = 0;
+  const long stepA = ACOL ? (long)BK * p.lda : 128, stepB = BCOL ? (long)BK * p.ldb : 128;
+  auto start = [&]() {
+    int tm, tn;
+    const int t = du / p.parts, part = du - t * p.parts;
+    tile_of(t, p.ntm, p.ntn, tm, tn);
+    dkt = part * per;
+    dend = min(dkt + per, p.nk);
+    const long oa = (ACOL ? (long)tm * C::BM * ES : (long)tm * C::BM * p.lda) + dkt * stepA;
+    long ob;
+    if constexpr (BCOL) ob = (long)tn * C::BN * ES + dkt * stepB;
+    else ob = epi.template first<C>(tn) * p.ldb + dkt * stepB;
+    dA = p.A + oa;
+    dB = p.B + ob;
+    lA = p.abytes - oa;
+    lB = p.bbytes - ob;
+  };
+  i32x4 ra, rb;
+  uint32_t dlds = 0;
+  auto aim = [&]() {                                            // past the end of the stream: reads nothing
+    const bool live = du < units;
+    ra = descriptor(dA, live ? lA : 0);
+    rb = descriptor(dB, live ? lB : 0);
+    dlds = lds0 + dslot * C::STAGE;
+  };
+  auto piece = [&](int q) {                                     // q: a constant once unrolled
+    const bool isA = q < C::A_LD, col = isA ? ACOL : BCOL;
+    const uint32_t off = col || dkt * BK + kin < p.K ? offs[q] : OUTSIDE;
+    dma16(isA ? ra : rb, off, dlds + (isA ? 0 : C::A_BYTES) + (wave + (isA ? q : q - C::A_LD) * (C::NT / 64)) * 1024);
+  };
+  auto next = [&]() {
+    dslot = dslot + 1 == NS ? 0 : dslot + 1;
+    if (du >= units) return;
+    if (++dkt < dend) {
+      dA += stepA;
+      lA -= stepA;
+      dB += stepB;
+      lB -= stepB;
+    } else {
+      du += gridDim.x;
+      if (du < units) start();
+    }
+  };
 
   // the lane's 16-byte chunk of k (step ks) of row `row0 + fr` of an operand image
   auto frag = [&](const char* im, int row0, int ks, auto COL_, auto RB_) -> i32x4 {
     constexpr bool COL = decltype(COL_)::value;
-    constexpr int rb = decltype(RB_)::value;           // bytes of an image row
+    constexpr int rowb = decltype(RB_)::value;
     if constexpr (!COL) {
       const int r = row0 + fr;
       return *reinterpret_cast<const i32x4*>(im + r * 128 + (((ks * 4 + fq) ^ (r & 7)) << 4));
@@ -206,7 +232,7 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = ks * 32 + fq * 8 + h * 4 + q, col = row0 + c * 4;
-        const char* at = im + r * rb + (((col >> 3) ^ col_swz<T, rb>(r)) << 4) + ((col >> 2) & 1) * 8;
+        const char* at = im + r * rowb + (((col >> 3) ^ col_swz<T, rowb>(r)) << 4) + ((col >> 2) & 1) * 8;
         v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(las_ptr)at);
       }
       return __builtin_bit_cast(i32x4, s16x8{v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w});
@@ -215,38 +241,103 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int r = ks * 16 + fq * 4 + s, col = row0 + fr;
-        v[s] = *reinterpret_cast<const int*>(im + r * rb + (((col >> 2) ^ col_swz<T, rb>(r)) << 4) + (col & 3) * 4);
+        v[s] = *reinterpret_cast<const int*>(im + r * rowb + (((col >> 2) ^ col_swz<T, rowb>(r)) << 4) + (col & 3) * 4);
       }
       return v;
     }
   };
-
-#pragma unroll
-  for (int t = 0; t < NS - 1; ++t)
-    if (k0 + t < k1) issue(k0 + t);
-  for (int kt = k0; kt < k1; ++kt) {
-    const int later = min(k1 - 1 - kt, NS - 2);                 // stages issued after this one
-    if (NS > 3 && later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::LD) : "memory");
-    else if (NS > 2 && later == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::LD) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (kt + NS - 1 < k1) issue(kt + NS - 1);
-    const char* ia = smem + ((kt - k0) % NS) * C::STAGE;
+  struct Frags { i32x4 a[TM], b[TN]; };
+  auto read = [&](Frags& f, int slot, int ks) {
+    const char* ia = smem + slot * C::STAGE;
     const char* ib = ia + C::A_BYTES;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      i32x4 fa[TM], fb[TN];
+    for (int j = 0; j < TN; ++j)
+      f.b[j] = frag(ib, wn * C::WN + j * 16, ks, std::integral_constant<bool, BCOL>{}, std::integral_constant<int, BRB>{});
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = frag(ib, wn * C::WN + j * 16, ks, std::integral_constant<bool, BCOL>{}, std::integral_constant<int, BRB>{});
+    for (int i = 0; i < TM; ++i)
+      f.a[i] = frag(ia, wm * C::WM + i * 16, ks, std::integral_constant<bool, ACOL>{}, std::integral_constant<int, ARB>{});
+  };
+  acc_t acc[TM][TN];
+  auto clear = [&]() {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = frag(ia, wm * C::WM + i * 16, ks, std::integral_constant<bool, ACOL>{}, std::integral_constant<int, ARB>{});
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int j = 0; j < TN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+  };
+  constexpr int PER = 2 * ((C::LD + TM - 1) / TM);              // pieces behind a row of MFMAs: the first half of the rows
+  auto mul = [&](const Frags& f, auto ISSUE_) {
+    constexpr bool ISSUE = decltype(ISSUE_)::value;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = step<T>(fb[j], fa[i], acc[i][j]);
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = step<T>(f.b[j], f.a[i], acc[i][j]);
+      if constexpr (ISSUE) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = i * PER; q < (i + 1) * PER; ++q)
+          if (q < C::LD) piece(q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
+  };
+
+  start();
+#pragma unroll
+  for (int t = 0; t < NS; ++t) {
+    aim();
+#pragma unroll
+    for (int q = 0; q < C::LD; ++q) piece(q);
+    next();
   }
-  epi.template write<C>(acc, tm * C::BM + wm * C::WM + fr, tn, wn, fq);
+  Frags f0, f1;
+  clear();
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * C::LD) : "memory");
+  read(f0, 0, 0);
+  int slot = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int t = u / p.parts, part = u - t * p.parts;
+    const int n = min(per, p.nk - part * per);
+    for (int k = 0; k < n; ++k) {
+      read(f1, slot, 1);
+      mul(f0, std::false_type{});
+      // stages behind the next one may be in flight; an epilogue's stores only make the wait longer
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * C::LD) : "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      slot = slot + 1 == NS ? 0 : slot + 1;
+      aim();
+      if (k + 1 < n) read(f0, slot, 0);                         // at a tile's end behind the epilogue: its registers
+      __builtin_amdgcn_sched_barrier(0);
+      mul(f1, std::true_type{});
+      next();
+    }
+    int tm, tn;
+    tile_of(t, p.ntm, p.ntn, tm, tn);
+    epi.template write<C>(acc, tm * C::BM + wm * C::WM + fr, tn, wn, fq, part);
+    clear();
+    read(f0, slot, 0);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // no DMA outlives the workgroup's LDS
+}
+
+template <class K>
+static int slots_of(K* fn, int threads) {
+  int dev = 0, cus = 0, per = 0;
+  (void)hipGetDevice(&dev);
+  (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  (void)hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, reinterpret_cast<const void*>(fn), threads, 0);
+  return (cus > 0 ? cus : 1) * (per > 0 ? per : 1);
+}
+
+template <typename T, class C, bool AC, bool BC, class Epi>
+static int launch_tiles(Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
+  p.ntm = (int)((m + C::BM - 1) / C::BM);
+  p.ntn = (int)((n + C::BN - 1) / C::BN);
+  const long units = (long)p.ntm * p.ntn * p.parts;
+  if (units > 0x7fffffffL) { set_error("%s: too many tiles", name); return SVK_EUNSUPPORTED; }
+  static const int slots = slots_of(&tile_mm<T, C, AC, BC, Epi>, C::NT);
+  hipLaunchKernelGGL((tile_mm<T, C, AC, BC, Epi>), dim3((unsigned)(units < slots ? units : slots)), dim3(C::NT), 0, st, p, epi);
+  set_last_kernel(name);
+  return check_launch(name);
 }
 
 // 16 (or fewer, at the end) token rows against the weights: each weight value is read once, straight into
@@ -254,6 +345,7 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
 // blocks of 16 weight rows (the epilogue's map names them).  VEC: rows 16-byte aligned and whole 16-byte chunks;
 // otherwise chunks are put together value by value.
 constexpr int SK_WAVES = 8;
+constexpr int SKINNY_M = 32;
 
 template <typename T, bool VEC>
 __device__ __forceinline__ i32x4 load_chunk(const char* row, long kb, long kbytes) {
