@@ -29,7 +29,7 @@ __device__ __forceinline__ float glu_act(float g, int act) {
   }
   if (act == SVK_GLU_GELU) {
     if constexpr (sizeof(T) == 4) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-    else return gelu_fast(g);
+    else return gelu16(g);
   }
   return g > 0.f ? g : (g <= 0.f ? 0.f : g);     // NaN stays NaN
 }
@@ -58,7 +58,7 @@ struct GateEpi {
   T* h; long ldh;
   T* pre;                 // [M, 2H] contiguous, or null
   const float* bias;      // [2H] or null
-  int M, H, act;
+  int M, H, act, per;
 
   __device__ __forceinline__ float activate(float g) const { return glu_act<T>(g, ACT < 0 ? act : ACT); }
   // a wave's columns: half gate, half up rows of the same hidden channels; the pairs of blocks interleaved where each
@@ -69,9 +69,14 @@ struct GateEpi {
     const int in = r % C::WN, up = in >= C::WN / 2, c = in - up * (C::WN / 2);
     return (uint32_t)(r / C::WN * (C::WN / 2) + (width<C>() == 8 ? pair_col(c) : c) + up * H) * ldb;
   }
-  __device__ __forceinline__ int skinny_row(int bid, int j, int fr) const { return min(bid * 16 + fr, H - 1) + j * H; }
+  // few tokens: `per` gate rows, then the up rows of the same channels
+  static constexpr bool PAIR = true;
+  __device__ __forceinline__ int skinny_row(int bid, int r) const {
+    const int up = r >= per;
+    return min(bid * per + min(r - up * per, per - 1), H - 1) + up * H;
+  }
   __device__ __forceinline__ void skinny_write(int bid, int m, int n, float g, float u) const {
-    const int c = bid * 16 + n;
+    const int c = bid * per + n;
     if (c >= H) return;
     if (bias) {
       g += bias[c];
@@ -158,14 +163,13 @@ __global__ __launch_bounds__(256) void join_parts(const float* __restrict__ S, i
 
 // dg, du from the kept projections: D [M][ld] = dg | du | zeros up to ld; S [row blocks][2H] = their column sums over
 // a block of rows, f32, before the rounding.  4 waves a workgroup, 64 * V columns, rows dealt to the waves in turn.
-constexpr int DP_ROWS = 64;
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, const T* __restrict__ dh, long lddh,
-                                                  T* __restrict__ D, long ld, float* __restrict__ S, int M, int H, int act) {
+                                                  T* __restrict__ D, long ld, float* __restrict__ S, int M, int H, int act, int rows) {
   __shared__ float sum[2][4][64 * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (blockIdx.y * 64 + lane) * V;
-  const long r0 = (long)blockIdx.x * DP_ROWS, r1 = min(r0 + DP_ROWS, (long)M);
+  const long r0 = (long)blockIdx.x * rows, r1 = min(r0 + rows, (long)M);
   const int nc = H - c;                       // columns that exist from c on (V divides H where V > 1)
   float sg[V], su[V];
 #pragma unroll
@@ -222,57 +226,28 @@ __global__ __launch_bounds__(256) void join_bias(const float* __restrict__ S, in
   }
 }
 
-using Big = Tile<256, 256, 2, 4, 2, 2>;
-using Mid = Tile<128, 128, 2, 2, 2, 2>;
-using Small = Tile<64, 64, 2, 2, 4, 2>;
+// rows a workgroup of gated_dpre: 64, fewer where that leaves CUs idle (16: 4 a wave)
+inline int dpre_rows(long m, long h) { return m * h >= 1L << 23 ? 64 : 16; }
 
-// tile choice: the largest tile that still gives the chip's 256 CUs most of a workgroup each
-inline int pick(long m, long n, long parts = 1) {
-  auto tiles = [&](long b) { return ((m + b - 1) / b) * ((n + b - 1) / b) * parts; };
-  if (tiles(256) >= 200) return 0;
-  if (tiles(128) >= 200) return 1;
-  return 2;
-}
-
-template <typename T, bool AC, bool BC, class Epi>
-static int tiled(int cfg, Args p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
-  p.nk = (p.K + 128 / (int)sizeof(T) - 1) / (128 / (int)sizeof(T));
-  if (cfg == 0) return launch_tiles<T, Big, AC, BC>(p, m, n, epi, st, name);
-  if (cfg == 1) return launch_tiles<T, Mid, AC, BC>(p, m, n, epi, st, name);
-  return launch_tiles<T, Small, AC, BC>(p, m, n, epi, st, name);
-}
-
-template <typename T, int MT, class Epi>
-static int skinny_mt(const Args& p, bool vec, int blocks, const Epi& epi, hipStream_t st) {
-  if (vec) hipLaunchKernelGGL((skinny_mm<T, MT, true, Epi>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
-  else hipLaunchKernelGGL((skinny_mm<T, MT, false, Epi>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
-  set_last_kernel("skinny_mm");
-  return check_launch("skinny_mm");
-}
-
-// the weight gradient's split of the token axis: small outputs would leave most CUs idle over a long reduction
-inline int dw_parts(long n2, long k, long m, int bk) {
-  const long tiles = ((n2 + 127) / 128) * ((k + 127) / 128);
-  const long nk = (m + bk - 1) / bk;
-  long parts = std::min<long>((512 + tiles - 1) / tiles, nk / 8);
-  parts = std::max<long>(1, std::min<long>(parts, 64));
-  const long per = (nk + parts - 1) / parts;
-  return (int)((nk + per - 1) / per);          // no empty part
-}
-
-// workspace of the backward pass: [dpre][x padded][w padded][bias partials][dw slabs]
+// workspace of the backward pass: [dpre][x padded][w padded][bias partials][slabs of dx, then of dw]
 struct BwdWs {
   long ldd, dpre, x, w, sums, slabs, total;
-  int parts;
-  BwdWs(long es, long M, long H, long K, bool padx, bool db, bool dw) {
+  int rows;
+  Plan px{2, 1}, pw{2, 1};
+  BwdWs(long es, long M, long H, long K, bool padx, bool db, bool dx, bool dw) {
+    auto plan = [&](long m, long n, long k) {
+      return es == 4 ? plan_tiles<float>(m, n, stages<float>(k), 64) : plan_tiles<bf16>(m, n, stages<bf16>(k), 64);
+    };
     ldd = up16(2 * H * es) / es;
     dpre = up16(M * ldd * es);
     const long ldk = up16(K * es);
     x = padx ? up16(M * ldk) : 0;
     w = padx ? up16(2 * H * ldk) : 0;
-    sums = db ? up16((M + DP_ROWS - 1) / DP_ROWS * 2 * H * 4) : 0;
-    parts = dw ? dw_parts(2 * H, K, M, 128 / (int)es) : 1;
-    slabs = parts > 1 ? up16(parts * 2 * H * K * 4) : 0;
+    rows = dpre_rows(M, H);
+    sums = db ? up16((M + rows - 1) / rows * 2 * H * 4) : 0;
+    if (dx) px = plan(M, K, 2 * H);
+    if (dw) pw = plan(2 * H, K, M);
+    slabs = std::max(px.parts > 1 ? up16(px.parts * M * K * 4) : 0, pw.parts > 1 ? up16(pw.parts * 2 * H * K * 4) : 0);
     total = dpre + x + w + sums + slabs;
   }
 };
@@ -328,9 +303,8 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(X, ldx, K, es) && rows_ok(W, ldw, K, es);
-      const int blocks = (int)((H + 15) / 16);
-      GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act};
-      return M <= 16 ? skinny_mt<T, 1>(p, vec, blocks, epi, st) : skinny_mt<T, 2>(p, vec, blocks, epi, st);
+      GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0};
+      return few_tokens<T, 2>(p, vec, H, epi, st, "gated_ffn_few");
     }
     char* at = (char*)ws;
     if (!rows_ok(X, ldx, K, es)) {
@@ -348,9 +322,11 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     }
     p.abytes = (M - 1) * p.lda + p.K * es;
     p.bbytes = (2 * H - 1) * p.ldb + p.K * es;
+    p.nk = stages<T>(p.K);
+    const int tile = plan_tiles<T>(M, 2 * H, p.nk, 1).tile;
     auto run = [&](auto act_c) {
-      GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act};
-      return tiled<T, false, false>(pick(M, 2 * H), p, M, 2 * H, epi, st, "gated_ffn");
+      GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0};
+      return launch_plan<T, false, false>(tile, p, M, 2 * H, epi, st, "gated_ffn");
     };
     if (act == SVK_GLU_SILU) return run(std::integral_constant<int, SVK_GLU_SILU>{});
     if (act == SVK_GLU_GELU) return run(std::integral_constant<int, SVK_GLU_GELU>{});
@@ -359,11 +335,11 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
 }
 
 extern "C" long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H,
-                                            long K, int want_dw, int want_db) {
+                                            long K, int want_dx, int want_dw, int want_db) {
   const long es = es_of(dtype);
   if (!es || bad_dims(M, H, K) || M == 0) return 0;
   const bool padx = !rows_ok(X, ldx, K, es) || !rows_ok(W, ldw, K, es);
-  return BwdWs(es, M, H, K, padx, want_db, want_dw).total;
+  return BwdWs(es, M, H, K, padx, want_db, want_dx, want_dw).total;
 }
 
 extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre,
@@ -382,7 +358,7 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     return SVK_EUNSUPPORTED;
   }
   const bool padx = !rows_ok(X, ldx, K, es) || !rows_ok(W, ldw, K, es);
-  const BwdWs need(es, M, H, K, padx, db, dW);
+  const BwdWs need(es, M, H, K, padx, db, dX, dW);
   if (M && (!ws || !al16(ws) || ws_bytes < need.total)) { set_error("svk_gated_ffn_bwd: workspace too small or misaligned"); return SVK_EINVAL; }
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
@@ -415,40 +391,38 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     }
     float* sums = db ? (float*)at : nullptr;
     at += need.sums;
-    float* slabs = need.parts > 1 ? (float*)at : nullptr;
-    const int rowblocks = (int)((M + DP_ROWS - 1) / DP_ROWS);
+    const int rowblocks = (int)((M + need.rows - 1) / need.rows);
     constexpr int V = 16 / (int)sizeof(T);
     auto al = [&](const void* q) { return ((uintptr_t)q & 15) == 0; };
     if (H % V == 0 && lddh % V == 0 && al(pre) && al(dH)) {
       hipLaunchKernelGGL((gated_dpre<T, V>), dim3(rowblocks, (unsigned)((H + 64 * V - 1) / (64 * V))), dim3(256), 0, st,
-                         (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act);
+                         (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
     } else {
       hipLaunchKernelGGL((gated_dpre<T, 1>), dim3(rowblocks, (unsigned)((H + 63) / 64)), dim3(256), 0, st, (const T*)pre,
-                         (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act);
+                         (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
     }
     if (int rc = check_launch("gated_dpre")) return rc;
     if (db) {
       hipLaunchKernelGGL(join_bias, dim3((unsigned)((2 * H + 15) / 16)), dim3(256), 0, st, sums, rowblocks, db, (int)(2 * H));
       if (int rc = check_launch("join_bias")) return rc;
     }
-    if (dX) {
-      PlainEpi<T> epi{(T*)dX, lddx, nullptr, (int)M, (int)K};
-      // the padding of D is zero and rows of W past 2H read as zero, so the reduction runs over whole chunks
-      Args p{(const char*)D, Wr, need.ldd * es, ldwb, M * need.ldd * es, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1};
-      if (int rc = tiled<T, false, true>(pick(M, K), p, M, K, epi, st, "gated_ffn_dx")) return rc;
-    }
-    if (dW) {
-      PlainEpi<T> epi{(T*)dW, K, slabs, (int)(2 * H), (int)K};
-      Args p{(const char*)D, Xr, need.ldd * es, ldxb, M * need.ldd * es, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, need.parts};
-      const int cfg = need.parts > 1 ? 1 : pick(2 * H, K);
-      if (int rc = tiled<T, true, true>(cfg, p, 2 * H, K, epi, st, "gated_ffn_dw")) return rc;
-      if (slabs) {
-        const long total = 2 * H * K;
-        hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((total + 255) / 256, 8192)), dim3(256), 0, st, slabs,
-                           need.parts, (T*)dW, K, (int)(2 * H), (int)K);
-        return check_launch("join_parts");
-      }
-    }
+    // y [m, n], of parts joined where the output has few tiles
+    auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, const char* name) -> int {
+      p.nk = stages<T>(p.K);
+      p.parts = plan.parts;
+      PlainEpi<T> epi{y, ldy, p.parts > 1 ? (float*)at : nullptr, (int)m, (int)n};
+      if (int rc = launch_plan<T, decltype(ac)::value, true>(plan.tile, p, m, n, epi, st, name)) return rc;
+      if (p.parts == 1) return SVK_OK;
+      hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((m * n + 255) / 256, 8192)), dim3(256), 0, st,
+                         (float*)at, p.parts, y, ldy, (int)m, (int)n);
+      return check_launch("join_parts");
+    };
+    const long Db = M * need.ldd * es;
+    // the padding of D is zero and rows of W past 2H read as zero, so dx's reduction runs over whole chunks
+    if (dX)
+      if (int rc = product(std::false_type{}, need.px, Args{(const char*)D, Wr, need.ldd * es, ldwb, Db, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1}, (T*)dX, lddx, M, K, "gated_ffn_dx")) return rc;
+    if (dW)
+      return product(std::true_type{}, need.pw, Args{(const char*)D, Xr, need.ldd * es, ldxb, Db, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, 1}, (T*)dW, K, 2 * H, K, "gated_ffn_dw");
     return SVK_OK;
   });
 }

@@ -1,7 +1,7 @@
 // Matrix product in 8-bit integers with a scale for each token and each output channel (svk_gemm_i8), and the
 // quantisation of token rows that feeds it (svk_quant_rows):
 //
-//   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] / s[m])            (ties to even; a row of zeros: s = 0, q = 0)
+//   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] * (127 / max))      (ties to even; a row of zeros: s = 0, q = 0)
 //   C[m, n] = act((sum_k qa[m, k] qw[n, k]) sa[m] sw[n] + bias[n]) + R[m, n]
 //
 // The integer sums are exact (int32: K <= 131072 for codes of -128 .. 127); everything behind them is f32, rounded once.
@@ -15,100 +15,151 @@ namespace svk {
 namespace i8 {
 using namespace mm;
 
-// one wave a row; NCH chunks of 8 values a lane kept in registers (0: read twice)
-template <typename T, int NCH, bool VEC>
+// largest of the 64 lanes' values, in every lane
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  auto over = [&](auto C) { v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(C)::value, 0xF, 0xF, true)); };
+  over(std::integral_constant<int, 0xB1>{});                    // lanes 1 0 3 2 of each four
+  over(std::integral_constant<int, 0x4E>{});                    // lanes 2 3 0 1
+  over(std::integral_constant<int, 0x141>{});                   // each eight mirrored
+  over(std::integral_constant<int, 0x140>{});                   // each sixteen mirrored
+  return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+             max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// RW rows a wave, read before the first is reduced; NCH chunks of 8 values a lane and row kept in registers (0: read
+// twice).
+// The largest magnitude is found on the bits without the sign, whose order as integers is that of the magnitudes (an
+// infinity or a NaN comes out largest).  A code is the product with 127 / max and 1.5 * 2^23 added in one fma: the sum's
+// last byte is the nearest integer to the exact product, ties to even.  (Three instructions a value; a division, a
+// rounding and two clamps each took 12544 rows of 512 f16 11.0 us, and this QRN.)
+template <typename T, int NCH, int RW, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long ldx, int8_t* __restrict__ Q, long ldq,
                                                   float* __restrict__ S, long M, int K) {
   const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= M) return;
-  const T* x = X + row * ldx;
-  int8_t* q = Q + row * ldq;
-  float top = 0.f;
-  bool fine = true;
-  auto see = [&](float v) {
-    top = fmaxf(top, fabsf(v));
-    fine = fine && fabsf(v) < INFINITY;
+  const long row0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RW;
+  if (row0 >= M) return;
+  constexpr int W = 2 * sizeof(T);                              // words of 8 values
+  float s, inv;
+  // the scale from the largest magnitude; inv = 127 / max, or 0 where that is no finite number: then codes come from a
+  // division (rows of subnormal values) or are 0
+  auto scale = [&](long row, float top) {
+    s = top < INFINITY ? top / 127.f : NAN;
+    inv = 127.f / top;
+    if (!(inv < INFINITY) || !(top < INFINITY)) inv = 0.f;
+    if (lane == 0) S[row] = s;
   };
-  auto code = [&](float v, float s) { return (int)rintf(fminf(fmaxf(v / s, -127.f), 127.f)); };
+  auto code = [&](float v) -> uint32_t {
+    if (inv > 0.f) return __float_as_uint(fmaf(v, inv, 12582912.f)) & 255u;
+    if (s > 0.f) return (uint32_t)(int)rintf(fminf(fmaxf(v / s, -127.f), 127.f)) & 255u;
+    return 0u;
+  };
   if constexpr (VEC) {
     const int nch = K >> 3;
-    float v[NCH > 0 ? NCH : 1][8];
-    auto load = [&](int ch, float* o) {
-      T t[8];
+    uint32_t v[RW][NCH > 0 ? NCH : 1][W], top[W];
+    auto load = [&](long row, int ch, uint32_t* o) {
 #pragma unroll
-      for (int p = 0; p < (int)sizeof(T) / 2; ++p)
-        reinterpret_cast<uint4*>(t)[p] = reinterpret_cast<const uint4*>(x + (long)ch * 8)[p];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = to_f(t[e]);
+      for (int p = 0; p < W / 4; ++p)
+        reinterpret_cast<uint4*>(o)[p] = reinterpret_cast<const uint4*>(X + row * ldx + (long)ch * 8)[p];
     };
-    if constexpr (NCH > 0) {
+    auto see = [&](const uint32_t* o) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
-        if (lane + 64 * i < nch) {
-          load(lane + 64 * i, v[i]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) see(v[i][e]);
-        }
-    } else {
-      for (int ch = lane; ch < nch; ch += 64) {
-        load(ch, v[0]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) see(v[0][e]);
+      for (int w = 0; w < W; ++w) {
+        if constexpr (sizeof(T) == 2)
+          top[w] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top[w]), __builtin_bit_cast(u16x2, o[w] & 0x7FFF7FFFu)));
+        else top[w] = max(top[w], o[w] & 0x7FFFFFFFu);
       }
-    }
-    top = wave_max(top);
-    fine = __all(fine);
-    const float s = fine ? top / 127.f : NAN;
-    if (lane == 0) S[row] = s;
-    auto store = [&](int ch, const float* o) {
-      uint32_t w[2] = {0u, 0u};
-      if (s > 0.f)
+    };
+    auto store = [&](long row, int ch, const uint32_t* o) {
+      uint32_t w[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= ((uint32_t)code(o[e], s) & 255u) << (8 * (e & 3));
-      *reinterpret_cast<uint2*>(q + (long)ch * 8) = uint2{w[0], w[1]};
+      for (int h = 0; h < 2; ++h) {
+        uint32_t c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f;
+          if constexpr (sizeof(T) == 4) f = __uint_as_float(o[h * 4 + e]);
+          else {
+            const f32x2 two = unpack2<T>(o[h * 2 + e / 2]);
+            f = e & 1 ? two.y : two.x;
+          }
+          c[e] = code(f);
+        }
+        w[h] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+      }
+      *reinterpret_cast<uint2*>(Q + row * ldq + (long)ch * 8) = uint2{w[0], w[1]};
     };
     if constexpr (NCH > 0) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
-        if (lane + 64 * i < nch) store(lane + 64 * i, v[i]);
-    } else {
-      for (int ch = lane; ch < nch; ch += 64) {
-        load(ch, v[0]);
-        store(ch, v[0]);
+      for (int r = 0; r < RW; ++r)
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (lane + 64 * i < nch) load(min(row0 + r, M - 1), lane + 64 * i, v[r][i]);
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const long row = row0 + r;
+      if (row >= M) return;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top[w] = 0u;
+      if constexpr (NCH > 0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (lane + 64 * i < nch) see(v[r][i]);
+      } else {
+        for (int ch = lane; ch < nch; ch += 64) {
+          load(row, ch, v[0][0]);
+          see(v[0][0]);
+        }
+      }
+      uint32_t m = 0u;
+#pragma unroll
+      for (int w = 0; w < W; ++w) m = max(m, sizeof(T) == 2 ? max(top[w] & 0xFFFFu, top[w] >> 16) : top[w]);
+      m = wave_umax(m);
+      if constexpr (sizeof(T) == 4) scale(row, __uint_as_float(m));
+      else scale(row, unpack2<T>(m).x);
+      if constexpr (NCH > 0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (lane + 64 * i < nch) store(row, lane + 64 * i, v[r][i]);
+      } else {
+        for (int ch = lane; ch < nch; ch += 64) {
+          load(row, ch, v[0][0]);
+          store(row, ch, v[0][0]);
+        }
       }
     }
   } else {
-    for (int k = lane; k < K; k += 64) see(to_f(x[k]));
-    top = wave_max(top);
-    fine = __all(fine);
-    const float s = fine ? top / 127.f : NAN;
-    if (lane == 0) S[row] = s;
-    for (int k = lane; k < K; k += 64) q[k] = s > 0.f ? (int8_t)code(to_f(x[k]), s) : 0;
+    static_assert(RW == 1, "rows of any alignment: one a wave");
+    const T* x = X + row0 * ldx;
+    uint32_t m = 0u;
+    for (int k = lane; k < K; k += 64) m = max(m, __float_as_uint(to_f(x[k])) & 0x7FFFFFFFu);
+    scale(row0, __uint_as_float(wave_umax(m)));
+    for (int k = lane; k < K; k += 64) Q[row0 * ldq + k] = (int8_t)code(to_f(x[k]));
   }
 }
 
-// ACT: none, GELU, or -1: `act`, chosen while running
+// ACT: none, GELU, ReLU, or -1: `act`, chosen while running
 template <typename T, int ACT>
 struct ScaleEpi {
   const float *sa, *sw, *bias;
   const T* R; long ldr;
   T* y; long ldy;
-  int M, N, act;
+  int M, N, act, per;
 
   __device__ __forceinline__ float value(int acc, float a, float w, float b) const {
     const float v = (float)acc * a * w + b;
     if constexpr (sizeof(T) == 4) return apply_act(v, ACT < 0 ? act : ACT);
+    else if constexpr (ACT == SVK_ACT_GELU) return gelu16(v);
     else return apply_act_fast(v, ACT < 0 ? act : ACT);
   }
   template <class C> __device__ __forceinline__ long first(int tn) const { return (long)tn * C::BN; }
   template <class C> __device__ __forceinline__ uint32_t offset(int r, uint32_t ldb) const { return (uint32_t)pair_col(r) * ldb; }
-  __device__ __forceinline__ int skinny_row(int bid, int j, int fr) const { return min(bid * 32 + j * 16 + fr, N - 1); }
-  __device__ __forceinline__ void skinny_write(int bid, int m, int n, int v0, int v1) const {
-    one(m, bid * 32 + n, v0);
-    one(m, bid * 32 + 16 + n, v1);
-  }
-  __device__ __forceinline__ void one(int m, int n, int acc) const {
+  static constexpr bool PAIR = false;
+  __device__ __forceinline__ int skinny_row(int bid, int r) const { return min(bid * per + min(r, per - 1), N - 1); }
+  __device__ __forceinline__ void skinny_write(int bid, int m, int i, int acc, int) const {
+    const int n = bid * per + i;
     if (n >= N) return;
     float v = value(acc, sa[m], sw[n], bias ? bias[n] : 0.f);
     if (R) v += to_f(R[(long)m * ldr + n]);
@@ -173,18 +224,6 @@ struct ScaleEpi {
   }
 };
 
-using Big = Tile<256, 256, 2, 4, 2, 2>;
-using Mid = Tile<128, 128, 2, 2, 2, 2>;
-using Small = Tile<64, 64, 2, 2, 4, 2>;
-template <typename T, int MT>
-static int go_skinny(const Args& p, bool vec, const ScaleEpi<T, -1>& epi, hipStream_t st) {
-  const int blocks = (epi.N + 31) / 32;
-  if (vec) hipLaunchKernelGGL((skinny_mm<int8_t, MT, true, ScaleEpi<T, -1>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
-  else hipLaunchKernelGGL((skinny_mm<int8_t, MT, false, ScaleEpi<T, -1>>), dim3(blocks), dim3(64 * SK_WAVES), 0, st, p, epi);
-  set_last_kernel("gemm_i8_skinny");
-  return check_launch("gemm_i8_skinny");
-}
-
 static bool rows_ok(const void* p, long ld, long K) { return al16(p) && ld % 16 == 0 && K % 16 == 0; }
 static bool bad_dims(long M, long N, long K) {
   return M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00L || N > 0x7fffff00L || K > 131072;
@@ -200,17 +239,27 @@ extern "C" int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long 
   if (M < 0 || K <= 0 || M > 0x7fffff00L || K > 0x7fffff00L || !X || !Q || !S || ldx < K || ldq < K) { set_error("svk_quant_rows: bad args"); return SVK_EINVAL; }
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)((M + 3) / 4)), block(256);
   SVK_DISPATCH_DTYPE(dtype, T, {
     const T* x = (const T*)X;
     int8_t* q = (int8_t*)Q;
+    auto go = [&](auto nch, auto rw, auto vec) {
+      constexpr int RW = decltype(rw)::value;
+      hipLaunchKernelGGL((quant_rows<T, decltype(nch)::value, RW, decltype(vec)::value>), dim3((unsigned)((M + 4 * RW - 1) / (4 * RW))),
+                         dim3(256), 0, st, x, ldx, q, ldq, S, M, (int)K);
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
     const bool vec = K % 8 == 0 && al16(X) && ldx * (long)sizeof(T) % 16 == 0 && ((uintptr_t)Q & 7) == 0 && ldq % 8 == 0;
-    if (!vec) hipLaunchKernelGGL((quant_rows<T, 0, false>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
-    else if (K <= 512) hipLaunchKernelGGL((quant_rows<T, 1, true>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
-    else if (K <= 1024) hipLaunchKernelGGL((quant_rows<T, 2, true>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
-    else if (K <= 2048) hipLaunchKernelGGL((quant_rows<T, 4, true>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
-    else if (K <= 4096) hipLaunchKernelGGL((quant_rows<T, 8, true>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
-    else hipLaunchKernelGGL((quant_rows<T, 0, true>), grid, block, 0, st, x, ldx, q, ldq, S, M, (int)K);
+    // short rows in numbers: several a wave, whose loads are under way together
+    const bool many = M >= 4096;
+    if (!vec) go(I0{}, I1{}, std::false_type{});
+    else if (K <= 512) many ? go(I1{}, I4{}, std::true_type{}) : go(I1{}, I1{}, std::true_type{});
+    else if (K <= 1024) many ? go(I2{}, I2{}, std::true_type{}) : go(I2{}, I1{}, std::true_type{});
+    else if (K <= 2048) go(I4{}, I1{}, std::true_type{});
+    else if (K <= 4096) go(std::integral_constant<int, 8>{}, I1{}, std::true_type{});
+    else go(I0{}, I1{}, std::true_type{});
     return check_launch("quant_rows");
   });
 }
@@ -241,8 +290,8 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
     Args p{(const char*)A, (const char*)W, lda, ldw, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(A, lda, K) && rows_ok(W, ldw, K);
-      ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act};
-      return M <= 16 ? go_skinny<T, 1>(p, vec, epi, st) : go_skinny<T, 2>(p, vec, epi, st);
+      ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0};
+      return few_tokens<int8_t, 1>(p, vec, N, epi, st, "gemm_i8_few");
     }
     char* at = (char*)ws;
     auto pad = [&](const void* X, long ld, long rows) {
@@ -263,18 +312,17 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
       p.ldb = ldk;
       p.K = (int)ldk;
     }
-    p.nk = (p.K + 127) / 128;
+    p.nk = stages<int8_t>(p.K);
     p.abytes = (M - 1) * p.lda + p.K;
     p.bbytes = (N - 1) * p.ldb + p.K;
-    auto tiles = [&](long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+    const int tile = plan_tiles<int8_t>(M, N, p.nk, 1).tile;
     auto run = [&](auto act_c) {
-      ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act};
-      if (tiles(256) >= 200) return launch_tiles<int8_t, Big, false, false>(p, M, N, epi, st, "gemm_i8");
-      if (tiles(128) >= 200) return launch_tiles<int8_t, Mid, false, false>(p, M, N, epi, st, "gemm_i8");
-      return launch_tiles<int8_t, Small, false, false>(p, M, N, epi, st, "gemm_i8");
+      ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0};
+      return launch_plan<int8_t, false, false>(tile, p, M, N, epi, st, "gemm_i8");
     };
     if (act == SVK_ACT_NONE) return run(std::integral_constant<int, SVK_ACT_NONE>{});
     if (act == SVK_ACT_GELU) return run(std::integral_constant<int, SVK_ACT_GELU>{});
+    if (act == SVK_ACT_RELU) return run(std::integral_constant<int, SVK_ACT_RELU>{});
     return run(std::integral_constant<int, -1>{});
   });
 }

@@ -139,6 +139,20 @@ __device__ __forceinline__ void put(T* at, const float* v, int n) {
 // position of tile-local B row r among the columns of its 32-column group: blocks of 16 interleaved by fours
 __device__ __forceinline__ int pair_col(int r) { return (r & ~31) + 8 * ((r >> 2) & 3) + 4 * ((r >> 4) & 1) + (r & 3); }
 
+// GELU (erf form) for results of 16 bits: relu(x) - |x| erfc(|x| / sqrt 2) / 2 with erfc by Abramowitz & Stegun 7.1.26
+// (|error| <= 1.5e-7): erfc(z) = t q(t) exp(-z^2), t = 1 / (1 + c z).  12 plain and 2 transcendental instructions; the
+// epilogues of short reductions are bound by them.
+__device__ __forceinline__ float gelu16(float x) {
+  constexpr float c = 0.3275911f * 0.70710678118654752f, s = -0.5f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(c, fabsf(x), 1.0f));
+  float q = fmaf(s * 1.061405429f, t, s * -1.453152027f);
+  q = fmaf(q, t, s * 1.421413741f);
+  q = fmaf(q, t, s * -0.284496736f);
+  q = fmaf(q, t, s * 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);                // -x^2 / 2 * log2(e)
+  return fmaf(fminf(fabsf(x), 1e4f) * t * q, e, x > 0.f ? x : 0.f);                     // bounded: infinity times t = 0
+}
+
 // Epi (row operand B): uint32_t offset<C>(r, ldb): bytes from the tile's first row to B row r of the tile;
 //                      long first<C>(tn): the tile's first row
 //      write<C>(acc, m, tn, wn, fq, part): stores the tile; acc[i][j]: row m + 16 i, columns 4 fq .. of block j
@@ -156,6 +170,7 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(las_ptr)smem;
   constexpr int ARB = ACOL ? C::BM * ES : 128, BRB = BCOL ? C::BN * ES : 128;      // image row bytes
   const int units = p.ntm * p.ntn * p.parts, per = (p.nk + p.parts - 1) / p.parts;
+  const int stride = gridDim.x;
   if ((int)blockIdx.x >= units) return;
 
   // DMA piece q of a stage: 1 KiB a wave of A's image, of B's from q = A_LD on
@@ -213,7 +228,7 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
       dB += stepB;
       lB -= stepB;
     } else {
-      du += gridDim.x;
+      du += stride;
       if (du < units) start();
     }
   };
@@ -294,15 +309,19 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * C::LD) : "memory");
   read(f0, 0, 0);
   int slot = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+  for (int u = blockIdx.x; u < units; u += stride) {
     const int t = u / p.parts, part = u - t * p.parts;
     const int n = min(per, p.nk - part * per);
     for (int k = 0; k < n; ++k) {
+      // the compiler counts LDS reads to 15 only: told that all of f0 (f1) has arrived, it does not wait for reads issued
+      // behind them (dx and dW, with 16 and 24 reads a step: DXA -> DXB, DWA -> DWB us)
+      __builtin_amdgcn_s_waitcnt(0xC07F);                       // lgkmcnt(0)
       read(f1, slot, 1);
       mul(f0, std::false_type{});
       // stages behind the next one may be in flight; an epilogue's stores only make the wait longer
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * C::LD) : "memory");
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      asm volatile("s_barrier" ::: "memory");
       slot = slot + 1 == NS ? 0 : slot + 1;
       aim();
       if (k + 1 < n) read(f0, slot, 0);                         // at a tile's end behind the epilogue: its registers
@@ -319,13 +338,50 @@ __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // no DMA outlives the workgroup's LDS
 }
 
+using Big = Tile<256, 256, 2, 4, 2, 2>;        // one workgroup a CU
+using Mid = Tile<128, 128, 2, 2, 2, 2>;        // two
+using Small = Tile<64, 64, 2, 2, 3, 3>;        // three
+
+// Which tile, and into how many parts the reduction is split where `most` allows it (parts are f32 slabs that another
+// kernel joins).  A CU works off its tiles at `step` us a stage with its residents together, but no stage of one tile in
+// less than `alone` us; `end` us a tile for its results.  Measured on 1 to 50176 rows, 96 to 5632 results, 64 to 2048
+// values of k; the choice is the best of the three, or within 10 % of it, at nearly all of them (1500 x 1024 x 2 x 5632
+// in bf16: 128-wide 50, 256-wide 57, 64-wide 68 us; 6000 x 2048 x 2 x 1024: 60, 51, 95; 100 x 2048 x 2 x 340: 24, 45, 14).
+struct Plan { int tile, parts; };
+struct Rate { double alone, step, end; };
+template <typename T>
+inline Plan plan_tiles(long m, long n, long nk, long most) {
+  constexpr Rate r16[3] = {{1.33, 1.5, 4.0}, {0.54, 0.47, 1.3}, {0.235, 0.2, 0.5}};
+  constexpr Rate r8[3] = {{1.1, 1.5, 8.0}, {0.5, 0.45, 2.2}, {0.21, 0.2, 0.7}};
+  constexpr Rate r32[3] = {{7.3, 7.3, 4.0}, {2.1, 2.0, 1.3}, {0.72, 0.54, 0.5}};
+  const Rate* rates = sizeof(T) == 4 ? r32 : (sizeof(T) == 1 ? r8 : r16);
+  Plan best{2, 1};
+  double least = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    const long side = 256 >> c;
+    const double tiles = (double)((m + side - 1) / side) * (double)((n + side - 1) / side);
+    for (long parts = 1; parts <= most && (parts == 1 || nk >= 4 * parts); parts *= 2) {
+      const long per = (nk + parts - 1) / parts, real = (nk + per - 1) / per;      // no empty part
+      const double each = ceil(tiles * (double)real / 256.0), k = (double)per;
+      double t = k * fmax(rates[c].alone, each * rates[c].step) + each * rates[c].end;
+      if (real > 1) t += 4.0 + (double)m * (double)n * 4.0 * (double)(real + 1) / 4e6;        // the slabs and their join
+      if (t < least) {
+        least = t;
+        best = Plan{c, (int)real};
+      }
+    }
+  }
+  return best;
+}
+
+struct Slots { int cus, per; };
 template <class K>
-static int slots_of(K* fn, int threads) {
+static Slots slots_of(K* fn, int threads) {
   int dev = 0, cus = 0, per = 0;
   (void)hipGetDevice(&dev);
   (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   (void)hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, reinterpret_cast<const void*>(fn), threads, 0);
-  return (cus > 0 ? cus : 1) * (per > 0 ? per : 1);
+  return Slots{cus > 0 ? cus : 1, per > 0 ? per : 1};
 }
 
 template <typename T, class C, bool AC, bool BC, class Epi>
@@ -334,18 +390,31 @@ static int launch_tiles(Args p, long m, long n, const Epi& epi, hipStream_t st, 
   p.ntn = (int)((n + C::BN - 1) / C::BN);
   const long units = (long)p.ntm * p.ntn * p.parts;
   if (units > 0x7fffffffL) { set_error("%s: too many tiles", name); return SVK_EUNSUPPORTED; }
-  static const int slots = slots_of(&tile_mm<T, C, AC, BC, Epi>, C::NT);
-  hipLaunchKernelGGL((tile_mm<T, C, AC, BC, Epi>), dim3((unsigned)(units < slots ? units : slots)), dim3(C::NT), 0, st, p, epi);
+  static const Slots slots = slots_of(&tile_mm<T, C, AC, BC, Epi>, C::NT);
+  const long all = (long)slots.cus * slots.per, grid = units < all ? units : all;
+  // a grid that does not fill the chip is spread over the CUs by asking for LDS that keeps the others off (left alone
+  // the dispatcher puts two workgroups on one CU beside idle ones: 176 tiles took as long as 352)
+  const long want = (grid + slots.cus - 1) / slots.cus, lds = (long)C::NS * C::STAGE;
+  long extra = 0;
+  if (want < slots.per) extra = ((160 * 1024 / (want + 1) + 512) / 512) * 512 - lds;
+  hipLaunchKernelGGL((tile_mm<T, C, AC, BC, Epi>), dim3((unsigned)grid), dim3(C::NT), (unsigned)(extra > 0 ? extra : 0), st, p, epi);
   set_last_kernel(name);
   return check_launch(name);
 }
+template <typename T, bool AC, bool BC, class Epi>
+static int launch_plan(int tile, const Args& p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
+  if (tile == 0) return launch_tiles<T, Big, AC, BC>(p, m, n, epi, st, name);
+  if (tile == 1) return launch_tiles<T, Mid, AC, BC>(p, m, n, epi, st, name);
+  return launch_tiles<T, Small, AC, BC>(p, m, n, epi, st, name);
+}
+template <typename T> inline int stages(long k) { return (int)((k * (long)sizeof(T) + 127) / 128); }
 
-// 16 (or fewer, at the end) token rows against the weights: each weight value is read once, straight into
-// registers, and the reduction is split over the workgroup's waves and joined in LDS.  MT blocks of 16 tokens, 2
-// blocks of 16 weight rows (the epilogue's map names them).  VEC: rows 16-byte aligned and whole 16-byte chunks;
-// otherwise chunks are put together value by value.
+// Few token rows against the weights: each weight value is read once, straight into registers, and the reduction is
+// split over the workgroup's waves and joined in LDS.  MT blocks of 16 tokens, NB blocks of 16 weight rows a workgroup
+// (the epilogue's map names them, `epi.per` results).  VEC: rows 16-byte aligned and whole 16-byte chunks; otherwise
+// chunks are put together value by value.  Bound by the weights' bytes, and below some MiB by one trip to memory.
 constexpr int SK_WAVES = 8;
-constexpr int SKINNY_M = 32;
+constexpr int SKINNY_M = 64;
 
 template <typename T, bool VEC>
 __device__ __forceinline__ i32x4 load_chunk(const char* row, long kb, long kbytes) {
@@ -353,7 +422,6 @@ __device__ __forceinline__ i32x4 load_chunk(const char* row, long kb, long kbyte
   if constexpr (VEC) {
     return kb < kbytes ? *reinterpret_cast<const i32x4*>(row + kb) : i32x4{0, 0, 0, 0};
   } else {
-    // 32-bit storage of the chunk's values, taken one by one
     union { i32x4 v; T e[16 / ES]; } u;
     u.v = i32x4{0, 0, 0, 0};
 #pragma unroll
@@ -363,33 +431,33 @@ __device__ __forceinline__ i32x4 load_chunk(const char* row, long kb, long kbyte
   }
 }
 
-template <typename T, int MT, bool VEC, class Epi>
+template <typename T, int MT, int NB, bool VEC, class Epi>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_mm(Args p, Epi epi) {
   typedef typename Acc<T>::t acc_t;
-  constexpr int U = VEC ? 4 : 1;                                // 64-byte steps in flight
+  constexpr int U = !VEC ? 1 : (MT + NB <= 2 ? 8 : (MT + NB <= 5 ? 4 : 2));        // 64-byte steps in flight
   typedef std::conditional_t<std::is_same<T, int8_t>::value, int, float> sum_t;
-  __shared__ sum_t red[SK_WAVES][MT][2][16][17];
+  __shared__ sum_t red[SK_WAVES][MT][NB][16][17];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int fr = lane & 15, fq = lane >> 4;
   const long kbytes = (long)p.K * sizeof(T);
-  const char* rb[2];
+  const char* rb[NB];
   const char* ra[MT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) rb[j] = p.B + (long)epi.skinny_row(blockIdx.x, j, fr) * p.ldb;
+  for (int j = 0; j < NB; ++j) rb[j] = p.B + (long)epi.skinny_row(blockIdx.x, j * 16 + fr) * p.ldb;
 #pragma unroll
   for (int i = 0; i < MT; ++i) ra[i] = p.A + (long)min(i * 16 + fr, p.M - 1) * p.lda;
-  acc_t acc[MT][2];
+  acc_t acc[MT][NB];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+    for (int j = 0; j < NB; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
   for (long kb = (long)wave * 64 * U; kb < kbytes; kb += (long)SK_WAVES * 64 * U) {
-    i32x4 fb[U][2], fa[U][MT];
+    i32x4 fb[U][NB], fa[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long k = kb + u * 64 + fq * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fb[u][j] = load_chunk<T, VEC>(rb[j], k, kbytes);
+      for (int j = 0; j < NB; ++j) fb[u][j] = load_chunk<T, VEC>(rb[j], k, kbytes);
 #pragma unroll
       for (int i = 0; i < MT; ++i) fa[u][i] = load_chunk<T, VEC>(ra[i], k, kbytes);
     }
@@ -398,24 +466,55 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_mm(Args p, Epi epi) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = step<T>(fb[u][j], fa[u][i], acc[i][j]);
+        for (int j = 0; j < NB; ++j) acc[i][j] = step<T>(fb[u][j], fa[u][i], acc[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) red[wave][i][j][fr][fq * 4 + e] = acc[i][j][e];
   __syncthreads();
-  for (int t = tid; t < MT * 256; t += 64 * SK_WAVES) {
-    const int i = t >> 8, m = (t >> 4) & 15, n = t & 15;
-    sum_t v[2] = {0, 0};
+  auto sum = [&](int m, int r) {                                // the waves' parts, in order
+    sum_t v = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int w = 0; w < SK_WAVES; ++w) v[j] += red[w][i][j][m][n];
-    if (i * 16 + m < p.M) epi.skinny_write(blockIdx.x, i * 16 + m, n, v[0], v[1]);
+    for (int w = 0; w < SK_WAVES; ++w) v += red[w][m >> 4][r >> 4][m & 15][r & 15];
+    return v;
+  };
+  for (int t = tid; t < p.M * epi.per; t += 64 * SK_WAVES) {
+    const int m = t / epi.per, n = t - m * epi.per;
+    epi.skinny_write(blockIdx.x, m, n, sum(m, n), Epi::PAIR ? sum(m, n + epi.per) : sum_t(0));
   }
+}
+
+// `results` of a row, epi.per a workgroup and WPR weight rows each: as many as give the 256 CUs one workgroup each (the
+// tokens are read once a workgroup, the weights evenly), 16 to 64 weight rows
+// (2 x 5632 rows of 2048 in bf16, 16 tokens: 32 rows a workgroup 15.5, 16 rows 13.9, 44 rows SKN us)
+template <typename T, int MT, int WPR, class Epi>
+static int launch_skinny(const Args& p, bool vec, long results, Epi epi, hipStream_t st, const char* name) {
+  long per = (results + 255) / 256;
+  per = per < 16 / WPR ? 16 / WPR : (per > 64 / WPR ? 64 / WPR : per);
+  epi.per = (int)per;
+  const dim3 grid((unsigned)((results + per - 1) / per)), block(64 * SK_WAVES);
+  auto go = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    if (vec) hipLaunchKernelGGL((skinny_mm<T, MT, NB, true, Epi>), grid, block, 0, st, p, epi);
+    else hipLaunchKernelGGL((skinny_mm<T, MT, NB, false, Epi>), grid, block, 0, st, p, epi);
+    set_last_kernel(name);
+    return check_launch(name);
+  };
+  switch ((per * WPR + 15) / 16) {
+    case 1: return go(std::integral_constant<int, 1>{});
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 3: return go(std::integral_constant<int, 3>{});
+    default: return go(std::integral_constant<int, 4>{});
+  }
+}
+template <typename T, int WPR, class Epi>
+static int few_tokens(const Args& p, bool vec, long results, const Epi& epi, hipStream_t st, const char* name) {
+  if (p.M <= 16) return launch_skinny<T, 1, WPR>(p, vec, results, epi, st, name);
+  if (p.M <= 32) return launch_skinny<T, 2, WPR>(p, vec, results, epi, st, name);
+  return launch_skinny<T, 4, WPR>(p, vec, results, epi, st, name);
 }
 
 // copy of rows of `width` values into rows of `ld` values (a multiple of 16 bytes), the rest filled with zeros: what

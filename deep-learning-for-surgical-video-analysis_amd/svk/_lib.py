@@ -132,7 +132,7 @@ LONG_FUNCS = {"svk_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int,
               "svk_mstcn_bwd_workspace": [c_int, c_int],
               "svk_stats_ws_floats": [c_int, c_int],
               "svk_gated_ffn_workspace": [c_int, P, c_long, P, c_long, c_long, c_long, c_long],
-              "svk_gated_ffn_bwd_workspace": [c_int, P, c_long, P, c_long, c_long, c_long, c_long, c_int, c_int],
+              "svk_gated_ffn_bwd_workspace": [c_int, P, c_long, P, c_long, c_long, c_long, c_long, c_int, c_int, c_int],
               "svk_gemm_i8_workspace": [P, c_long, P, c_long, c_long, c_long, c_long]}
 INT_QUERIES = {"svk_mixffn_supported": [c_int, c_int], "svk_mixffn_rw_supported": [c_int, c_int, c_int],
                "svk_mixffn_dw_fc2_supported": [c_int, c_int, c_int, c_int],

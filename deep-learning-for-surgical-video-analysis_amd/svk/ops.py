@@ -1477,36 +1477,62 @@ def mstcn_bwd_floats(T, F):
 
 
 # ---- token-block operators: rotary positions over (time, height, width), gated feed-forward, 8-bit products
+# A pass over a few tokens takes the GPU 3 to 5 us, less than the checks, allocations and the launch take the host:
+# these wrappers look every property of a tensor up once, compare device numbers, and ask torch for the raw stream
+# (0.07 us; the Stream object costs 2.5).  rope3d of one token 16.2 -> 8.5 us a call.
 
 GLU_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 _POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
 
-def _same_device(fn, first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise _lib.SvkError(f"svk.{fn}: tensors on {first.device} and {t.device}")
+def _code(t, fn, name):
+    """(dtype code, device number) of an operator's first tensor."""
+    dt = _DT.get(t.dtype)
+    if dt is None:
+        raise _lib.SvkError(f"svk.{fn}: unsupported dtype {t.dtype} (float32 / float16 / bfloat16 only)")
+    dev = t.get_device()
+    if dev < 0:
+        raise _lib.SvkError(f"svk.{fn}: {name} must be a GPU tensor (got {t.device}); there is no CPU path")
+    return dt, dev
 
 
-def _on(first, name, *args):
-    """The library call on ``first``'s device and that device's current stream."""
-    i = first.device.index
-    if i == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+def _like(t, dtype, dev, fn, name):
+    """The tensor has this dtype and lies on this device."""
+    if t.dtype is not dtype:
+        raise _lib.SvkError(f"svk.{fn}: {name} dtype {t.dtype} != {dtype}")
+    if t.get_device() != dev:
+        raise _lib.SvkError(f"svk.{fn}: {name} must be on the GPU {dev} (got {t.device}); there is no CPU path")
+
+
+def _on(dev, call, *args):
+    """The library call on device ``dev`` and that device's current stream."""
+    if dev == _current_device():
+        rc = call(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(i):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            rc = call(*args, _raw_stream(dev))
+    if rc:
+        raise _lib.SvkError(f"{call.__name__} failed ({rc}): {_lib.load().svk_last_error().decode()}")
 
 
 def _token_rows(t, fn, name):
     """(rows, columns, row stride) of a [..., C] tensor whose leading dims are one even run of rows; dims of one
     element do not count (the newest token x[:, -1:] of a batch is such a run)."""
-    cols = t.shape[-1] if t.dim() else 0
-    if cols == 0 or (cols > 1 and t.stride(-1) != 1):
-        raise _lib.SvkError(f"svk.{fn}: {name} {tuple(t.shape)} must have a last dim of unit stride")
-    rows, ld, run = t.numel() // cols, None, None
-    if rows > 1:
-        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    shape = t.shape
+    cols = shape[-1] if shape else 0
+    stride = t.stride()
+    if cols == 0 or (cols > 1 and stride[-1] != 1):
+        raise _lib.SvkError(f"svk.{fn}: {name} {tuple(shape)} must have a last dim of unit stride")
+    rows = t.numel() // cols
+    if rows <= 1:
+        return rows, cols, cols
+    if len(shape) == 2:
+        ld = stride[0]
+    else:
+        ld = None
+        for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
             if n == 1:
                 continue
             if ld is None:
@@ -1514,17 +1540,15 @@ def _token_rows(t, fn, name):
             elif s != run:
                 raise _lib.SvkError(f"svk.{fn}: {name} leading dims are not uniformly strided")
             run *= n
-    ld = cols if ld is None else ld
-    if rows > 1 and ld < cols:
+    if ld < cols:
         raise _lib.SvkError(f"svk.{fn}: {name} rows overlap (stride {ld} < {cols} columns)")
     return rows, cols, ld
 
 
-def _vector(t, n, fn, name):
-    if t is not None:
-        _chk(t, name, torch.float32)
-        if t.numel() != n or not t.is_contiguous():
-            raise _lib.SvkError(f"svk.{fn}: {name} must be {n} contiguous float32 values, got {tuple(t.shape)}")
+def _vector(t, n, dev, fn, name):
+    _like(t, torch.float32, dev, fn, name)
+    if t.numel() != n or not t.is_contiguous():
+        raise _lib.SvkError(f"svk.{fn}: {name} must be {n} contiguous float32 values, got {tuple(t.shape)}")
 
 
 def _apart(a, b):
@@ -1560,6 +1584,27 @@ def rope3d_freqs(sections, base=10000.0, shared=False, device="cuda"):
     return torch.pow(torch.tensor(float(base), dtype=torch.float64), -e).to(device)
 
 
+def _rope_out(q, k, out):
+    """The given outputs of rope3d, checked."""
+    qo, ko = out
+    if (ko is None) != (k is None):
+        raise _lib.SvkError("svk.rope3d: out must be (q', k') like (q, k)")
+    for o, t, nm in ((qo, q, "q"), (ko, k, "k")):
+        if t is None:
+            continue
+        _like(o, q.dtype, q.get_device(), "rope3d", "out")
+        if o.shape != t.shape:
+            raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
+        B, N, width = t.shape
+        sb, sn, sc = o.stride()
+        if (width > 1 and sc != 1) or (N > 1 and sn < width) or (B > 1 and sb < (sn * (N - 1) if N > 1 else 0) + width):
+            raise _lib.SvkError("svk.rope3d: out rows overlap or lack unit channel stride")
+    if not (_apart(qo, q) and _apart(qo, k) and _apart(ko, k) and _apart(ko, q) and _apart(qo, ko)) or \
+            (ko is not None and qo.data_ptr() == ko.data_ptr() and qo.numel()):
+        raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
+    return qo, ko
+
+
 def rope3d(q, k, pos, freqs, sections, heads, kv_heads=None, interleaved=False, inverse=False, out=None):
     """(q', k') with every head's pairs turned by the token's (time, row, column): svk_rope3d.
 
@@ -1567,74 +1612,73 @@ def rope3d(q, k, pos, freqs, sections, heads, kv_heads=None, interleaved=False, 
     [B, N, 3] int32 / int64 / float32; sections = pairs of the three axes, in this order, 2 * sum <= hd; freqs float64
     [sum(sections)] (rope3d_freqs).  ``inverse`` turns back: the gradient of the rotation.  ``out`` = (q', k') to write,
     which may be (q, k)."""
-    fn = "rope3d"
-    dt = dtype_code(q.dtype)
-    _chk(q, "q"); _chk(k, "k", q.dtype); _chk(pos, "pos"); _chk(freqs, "freqs", torch.float64)
-    kv_heads = 0 if k is None else heads if kv_heads is None else kv_heads
-    nt, nh, nw = sections
-    if q.dim() != 3 or heads < 1 or q.shape[2] % heads or q.shape[2] == 0:
-        raise _lib.SvkError(f"svk.rope3d: q {tuple(q.shape)} is not [B, N, {heads} * hd]")
-    B, N, C = q.shape
+    dt, dev = _code(q, "rope3d", "q")
+    shape = q.shape
+    if len(shape) != 3 or heads < 1 or shape[2] % heads or shape[2] == 0:
+        raise _lib.SvkError(f"svk.rope3d: q {tuple(shape)} is not [B, N, {heads} * hd]")
+    B, N, C = shape
     hd = C // heads
-    if k is not None and (kv_heads < 1 or k.shape != (B, N, kv_heads * hd)):
-        raise _lib.SvkError(f"svk.rope3d: k {tuple(k.shape)} is not [{B}, {N}, {kv_heads} * {hd}]")
-    if min(nt, nh, nw) < 0 or not 0 < 2 * (nt + nh + nw) <= hd:
+    nt, nh, nw = sections
+    R = nt + nh + nw
+    if nt < 0 or nh < 0 or nw < 0 or not 0 < 2 * R <= hd:
         raise _lib.SvkError(f"svk.rope3d: sections {tuple(sections)} do not fit a head of {hd}")
-    if freqs.shape != (nt + nh + nw,) or not freqs.is_contiguous():
-        raise _lib.SvkError(f"svk.rope3d: freqs must be {nt + nh + nw} contiguous float64 values")
-    if pos.dtype not in _POS or pos.shape not in ((N, 3), (B, N, 3)) or pos.stride(-1) != 1:
+    _like(freqs, torch.float64, dev, "rope3d", "freqs")
+    if freqs.shape != (R,) or not freqs.is_contiguous():
+        raise _lib.SvkError(f"svk.rope3d: freqs must be {R} contiguous float64 values")
+    ptype, pshape, pst = _POS.get(pos.dtype), pos.shape, pos.stride()
+    if ptype is None or (pshape != (B, N, 3) and pshape != (N, 3)) or pst[-1] != 1:
         raise _lib.SvkError(f"svk.rope3d: pos must be [N, 3] or [B, N, 3] int32 / int64 / float32 of unit stride, got "
-                            f"{tuple(pos.shape)} {pos.dtype}")
-    if out is None:
-        qo = torch.empty(B, N, C, device=q.device, dtype=q.dtype)
-        ko = None if k is None else torch.empty(B, N, kv_heads * hd, device=q.device, dtype=q.dtype)
+                            f"{tuple(pshape)} {pos.dtype}")
+    _like(pos, pos.dtype, dev, "rope3d", "pos")
+    qs = q.stride()
+    if C > 1 and qs[2] != 1:
+        raise _lib.SvkError("svk.rope3d: q must have unit channel stride")
+    if k is None:
+        kv_heads = 0
     else:
-        qo, ko = out
-        if (ko is None) != (k is None):
-            raise _lib.SvkError("svk.rope3d: out must be (q', k') like (q, k)")
-        for o, t, nm in ((qo, q, "q"), (ko, k, "k")):
-            if t is None:
-                continue
-            _chk(o, "out", q.dtype)
-            if o.shape != t.shape:
-                raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
-            width = t.shape[2]
-            if (N > 1 and o.stride(1) < width) or (B > 1 and o.stride(0) < (o.stride(1) * (N - 1) if N > 1 else 0) + width):
-                raise _lib.SvkError("svk.rope3d: out rows overlap")
-        if not (_apart(qo, q) and _apart(qo, k) and _apart(ko, k) and _apart(ko, q) and _apart(qo, ko)) or \
-                (ko is not None and qo.data_ptr() == ko.data_ptr() and qo.numel()):
-            raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
-    for t, nm in ((q, "q"), (k, "k"), (qo, "out"), (ko, "out")):
-        if t is not None and t.stride(2) != 1 and t.shape[2] > 1:
-            raise _lib.SvkError(f"svk.rope3d: {nm} must have unit channel stride")
-    _same_device(fn, q, k, pos, freqs, qo, ko)
+        kv_heads = heads if kv_heads is None else kv_heads
+        _like(k, q.dtype, dev, "rope3d", "k")
+        if kv_heads < 1 or k.shape != (B, N, kv_heads * hd):
+            raise _lib.SvkError(f"svk.rope3d: k {tuple(k.shape)} is not [{B}, {N}, {kv_heads} * {hd}]")
+        ks = k.stride()
+        if ks[2] != 1 and k.shape[2] > 1:
+            raise _lib.SvkError("svk.rope3d: k must have unit channel stride")
+    if out is None:
+        qo = torch.empty(shape, device=q.device, dtype=q.dtype)
+        qos = (N * C, C)
+        if k is None:
+            ko = None
+        else:
+            ko = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+            kos = (N * kv_heads * hd, kv_heads * hd)
+    else:
+        qo, ko = _rope_out(q, k, out)
+        qos = qo.stride()
+        kos = None if ko is None else ko.stride()
     if B * N:
-        s = lambda t: (None, 0, 0) if t is None else (t.data_ptr(), t.stride(1), t.stride(0))  # noqa: E731
-        _on(q, "svk_rope3d", dt, *s(q), *s(qo), heads, *s(k), *s(ko), kv_heads, pos.data_ptr(), _POS[pos.dtype],
-            pos.stride(-2), pos.stride(0) if pos.dim() == 3 else 0, freqs.data_ptr(), nt, nh, nw, hd, B, N,
-            int(interleaved), int(inverse))
+        kargs = (None, 0, 0, None, 0, 0, 0) if k is None else (k.data_ptr(), ks[1], ks[0], ko.data_ptr(), kos[1], kos[0],
+                                                               kv_heads)
+        _on(dev, _lib.load().svk_rope3d, dt, q.data_ptr(), qs[1], qs[0], qo.data_ptr(), qos[1], qos[0], heads, *kargs,
+            pos.data_ptr(), ptype, pst[-2], pst[0] if len(pst) == 3 else 0, freqs.data_ptr(), nt, nh, nw, hd, B, N,
+            1 if interleaved else 0, 1 if inverse else 0)
     return qo, ko
 
 
 def _glu(act, fn):
-    try:
-        return GLU_ACT[act]
-    except KeyError:
-        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(GLU_ACT)}") from None
+    code = GLU_ACT.get(act)
+    if code is None:
+        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(GLU_ACT)}")
+    return code
 
 
 def _gated_args(x, w, fn):
-    dt = dtype_code(x.dtype)
-    _chk(x, "x"); _chk(w, "w", x.dtype)
+    dt, dev = _code(x, fn, "x")
+    _like(w, x.dtype, dev, fn, "w")
     M, K, ldx = _token_rows(x, fn, "x")
-    if w.dim() != 2 or w.shape[1] != K or w.shape[0] % 2 or w.shape[0] == 0:
-        raise _lib.SvkError(f"svk.{fn}: w {tuple(w.shape)} is not [2 * hidden, {K}] (gate rows, then up rows)")
-    _, _, ldw = _token_rows(w, fn, "w")
-    return dt, M, K, ldx, ldw, w.shape[0] // 2
-
-
-def _bytes(n, like):
-    return torch.empty(n, device=like.device, dtype=torch.uint8) if n else None
+    ws = w.shape
+    if len(ws) != 2 or ws[1] != K or ws[0] % 2 or ws[0] == 0:
+        raise _lib.SvkError(f"svk.{fn}: w {tuple(ws)} is not [2 * hidden, {K}] (gate rows, then up rows)")
+    return dt, dev, M, K, ldx, _token_rows(w, fn, "w")[2], ws[0] // 2
 
 
 def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
@@ -1642,26 +1686,26 @@ def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
     bias = cat([bg, bu]) float32 or None, act "silu" / "gelu" / "relu" -> [..., hidden].  ``save`` returns (h, pre) with
     pre [..., 2 * hidden] the two projections, which gated_ffn_bwd reads.  The down projection is ``gemm``."""
     fn = "gated_ffn"
-    dt, M, K, ldx, ldw, H = _gated_args(x, w, fn)
+    dt, dev, M, K, ldx, ldw, H = _gated_args(x, w, fn)
     code = _glu(act, fn)
-    _vector(bias, 2 * H, fn, "bias")
+    if bias is not None:
+        _vector(bias, 2 * H, dev, fn, "bias")
     lead = x.shape[:-1]
     if out is None:
-        out, ldh = torch.empty(*lead, H, device=x.device, dtype=x.dtype), H
+        out, ldh = torch.empty((*lead, H), device=x.device, dtype=x.dtype), H
     else:
-        _chk(out, "out", x.dtype)
+        _like(out, x.dtype, dev, fn, "out")
         if out.shape != (*lead, H):
             raise _lib.SvkError(f"svk.{fn}: out is {tuple(out.shape)}, not {(*lead, H)}")
         _, _, ldh = _token_rows(out, fn, "out")
-        if not (_apart(out, x) and _apart(out, w)) or (M and out.data_ptr() in (x.data_ptr(), w.data_ptr())):
+        if not (_apart(out, x) and _apart(out, w) and _apart(out, bias)) or (M and out.data_ptr() in (x.data_ptr(), w.data_ptr())):
             raise _lib.SvkError(f"svk.{fn}: out overlaps an input")
-    pre = torch.empty(*lead, 2 * H, device=x.device, dtype=x.dtype) if save else None
-    _same_device(fn, x, w, bias, out)
+    pre = torch.empty((*lead, 2 * H), device=x.device, dtype=x.dtype) if save else None
     if M:
-        px, pw = x.data_ptr(), w.data_ptr()
-        nb = _lib.load().svk_gated_ffn_workspace(dt, px, ldx, pw, ldw, M, H, K)
-        ws = _bytes(nb, x)
-        _on(x, "svk_gated_ffn", dt, px, ldx, pw, ldw, _p(bias), out.data_ptr(), ldh, _p(pre), M, H, K, code, _p(ws), nb)
+        lib, px, pw = _lib.load(), x.data_ptr(), w.data_ptr()
+        nb = lib.svk_gated_ffn_workspace(dt, px, ldx, pw, ldw, M, H, K)
+        ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
+        _on(dev, lib.svk_gated_ffn, dt, px, ldx, pw, ldw, _p(bias), out.data_ptr(), ldh, _p(pre), M, H, K, code, _p(ws), nb)
     return (out, pre) if save else out
 
 
@@ -1669,47 +1713,44 @@ def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
     """Gradients (dx, dw, db) of gated_ffn from dh [..., hidden] and the saved ``pre``: dx like x, dw [2 * hidden, K] in
     w's dtype, db float32 [2 * hidden]; None where not asked for.  Written, not added to; the same bits on every run."""
     fn = "gated_ffn_bwd"
-    dt, M, K, ldx, ldw, H = _gated_args(x, w, fn)
+    dt, dev, M, K, ldx, ldw, H = _gated_args(x, w, fn)
     code = _glu(act, fn)
-    _chk(pre, "pre", x.dtype); _chk(dh, "dh", x.dtype)
+    _like(pre, x.dtype, dev, fn, "pre")
+    _like(dh, x.dtype, dev, fn, "dh")
     lead = x.shape[:-1]
     if pre.shape != (*lead, 2 * H) or not pre.is_contiguous():
         raise _lib.SvkError(f"svk.{fn}: pre {tuple(pre.shape)} is not contiguous {(*lead, 2 * H)}")
     if dh.shape != (*lead, H):
         raise _lib.SvkError(f"svk.{fn}: dh {tuple(dh.shape)} is not {(*lead, H)}")
     _, _, lddh = _token_rows(dh, fn, "dh")
-    _same_device(fn, x, w, pre, dh)
-    gx = torch.empty(*lead, K, device=x.device, dtype=x.dtype) if dx else None
-    gw = torch.empty(2 * H, K, device=x.device, dtype=x.dtype) if dw else None
+    gx = torch.empty((*lead, K), device=x.device, dtype=x.dtype) if dx else None
+    gw = torch.empty((2 * H, K), device=x.device, dtype=x.dtype) if dw else None
     gb = torch.empty(2 * H, device=x.device, dtype=torch.float32) if db else None
-    if (dx and M) or dw or db:
-        px, pw = x.data_ptr(), w.data_ptr()
-        nb = _lib.load().svk_gated_ffn_bwd_workspace(dt, px, ldx, pw, ldw, M, H, K, int(dw), int(db)) if M else 0
-        ws = _bytes(nb, x)
-        if M:
-            _on(x, "svk_gated_ffn_bwd", dt, px, ldx, pw, ldw, pre.data_ptr(), dh.data_ptr(), lddh, _p(gx), K, _p(gw),
-                _p(gb), M, H, K, code, _p(ws), nb)
-        else:
-            for t in (gw, gb):
-                if t is not None:
-                    t.zero_()
+    if M and (dx or dw or db):
+        lib, px, pw = _lib.load(), x.data_ptr(), w.data_ptr()
+        nb = lib.svk_gated_ffn_bwd_workspace(dt, px, ldx, pw, ldw, M, H, K, 1 if dx else 0, 1 if dw else 0, 1 if db else 0)
+        ws = torch.empty(nb, device=x.device, dtype=torch.uint8)
+        _on(dev, lib.svk_gated_ffn_bwd, dt, px, ldx, pw, ldw, pre.data_ptr(), dh.data_ptr(), lddh, _p(gx), K, _p(gw), _p(gb),
+            M, H, K, code, ws.data_ptr(), nb)
+    elif M == 0:
+        for t in (gw, gb):
+            if t is not None:
+                t.zero_()
     return gx, gw, gb
 
 
 def quant_rows(x):
-    """(codes int8 [..., K], scale float32 [...]) with x ~ codes * scale: scale = max |row| / 127, codes rounded to the
-    nearest, ties to even (svk_quant_rows).  Tokens before ``gemm_i8``; a weight [N, K] once, when it is loaded.  Rows of
-    the codes are 16 bytes apart at least (a view of a padded buffer where K % 16 != 0)."""
-    fn = "quant_rows"
-    dt = dtype_code(x.dtype)
-    _chk(x, "x")
-    M, K, ldx = _token_rows(x, fn, "x")
+    """(codes int8 [..., K], scale float32 [...]) with x ~ codes * scale: scale = max |row| / 127, codes
+    the integers nearest to x * (127 / max), ties to even (svk_quant_rows).  Tokens before ``gemm_i8``; a weight [N, K] once, when it is loaded.  Rows of
+    the codes are a multiple of 16 bytes apart (a view of a padded buffer where K % 16 != 0)."""
+    dt, dev = _code(x, "quant_rows", "x")
+    M, K, ldx = _token_rows(x, "quant_rows", "x")
     ldq = (K + 15) // 16 * 16
     lead = x.shape[:-1]
-    q = torch.empty(*lead, ldq, device=x.device, dtype=torch.int8)
+    q = torch.empty((*lead, ldq), device=x.device, dtype=torch.int8)
     s = torch.empty(lead, device=x.device, dtype=torch.float32)
     if M:
-        _on(x, "svk_quant_rows", dt, x.data_ptr(), ldx, q.data_ptr(), ldq, s.data_ptr(), M, K)
+        _on(dev, _lib.load().svk_quant_rows, dt, x.data_ptr(), ldx, q.data_ptr(), ldq, s.data_ptr(), M, K)
     return (q if ldq == K else q[..., :K]), s
 
 
@@ -1718,37 +1759,48 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, act=None, residual=None, out=None
     a_scale float32 [...], w int8 [N, K] with w_scale float32 [N] (both from quant_rows) -> [..., N] in ``dtype`` (or
     out's).  K <= 131072.  ``out`` may be ``residual``."""
     fn = "gemm_i8"
-    _chk(a, "a", torch.int8); _chk(w, "w", torch.int8)
+    dev = a.get_device()
+    if dev < 0:
+        raise _lib.SvkError(f"svk.{fn}: a must be a GPU tensor (got {a.device}); there is no CPU path")
+    _like(a, torch.int8, dev, fn, "a")
+    _like(w, torch.int8, dev, fn, "w")
     M, K, lda = _token_rows(a, fn, "a")
-    if w.dim() != 2 or w.shape[1] != K or w.shape[0] == 0:
-        raise _lib.SvkError(f"svk.{fn}: w {tuple(w.shape)} does not match K={K}")
-    _, _, ldw = _token_rows(w, fn, "w")
-    N = w.shape[0]
-    _vector(a_scale, M, fn, "a_scale"); _vector(w_scale, N, fn, "w_scale"); _vector(bias, N, fn, "bias")
+    wsh = w.shape
+    if len(wsh) != 2 or wsh[1] != K or wsh[0] == 0:
+        raise _lib.SvkError(f"svk.{fn}: w {tuple(wsh)} does not match K={K}")
+    ldw, N = _token_rows(w, fn, "w")[2], wsh[0]
+    _vector(a_scale, M, dev, fn, "a_scale")
+    _vector(w_scale, N, dev, fn, "w_scale")
+    if bias is not None:
+        _vector(bias, N, dev, fn, "bias")
+    code = ACT.get(act)
+    if code is None:
+        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(k for k in ACT if k)}")
     lead = a.shape[:-1]
     if out is None:
-        out, ldy = torch.empty(*lead, N, device=a.device, dtype=dtype), N
+        dt = _DT.get(dtype)
+        if dt is None:
+            raise _lib.SvkError(f"svk.{fn}: unsupported dtype {dtype} (float32 / float16 / bfloat16 only)")
+        out, ldy = torch.empty((*lead, N), device=a.device, dtype=dtype), N
     else:
-        _chk(out, "out")
+        dt, _ = _code(out, fn, "out")
+        dtype = out.dtype
+        _like(out, dtype, dev, fn, "out")
         if out.shape != (*lead, N):
             raise _lib.SvkError(f"svk.{fn}: out is {tuple(out.shape)}, not {(*lead, N)}")
         _, _, ldy = _token_rows(out, fn, "out")
-        if not (_apart(out, a) and _apart(out, w) and _apart(out, residual)):
+        if not all(_apart(out, t) for t in (a, a_scale, w, w_scale, bias, residual)):
             raise _lib.SvkError(f"svk.{fn}: out overlaps an input")
-    dt = dtype_code(out.dtype)
     ldr = 0
     if residual is not None:
-        _chk(residual, "residual", out.dtype)
+        _like(residual, dtype, dev, fn, "residual")
         if residual.shape != out.shape:
             raise _lib.SvkError(f"svk.{fn}: residual is {tuple(residual.shape)}, not {tuple(out.shape)}")
         _, _, ldr = _token_rows(residual, fn, "residual")
-    if act not in ACT:
-        raise _lib.SvkError(f"svk.{fn}: act {act!r} is none of {sorted(k for k in ACT if k)}")
-    _same_device(fn, a, a_scale, w, w_scale, bias, residual, out)
     if M:
-        pa, pw = a.data_ptr(), w.data_ptr()
-        nb = _lib.load().svk_gemm_i8_workspace(pa, lda, pw, ldw, M, N, K)
-        ws = _bytes(nb, a)
-        _on(a, "svk_gemm_i8", dt, pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), _p(bias), _p(residual), ldr,
-            out.data_ptr(), ldy, M, N, K, ACT[act], _p(ws), nb)
+        lib, pa, pw = _lib.load(), a.data_ptr(), w.data_ptr()
+        nb = lib.svk_gemm_i8_workspace(pa, lda, pw, ldw, M, N, K)
+        ws = torch.empty(nb, device=a.device, dtype=torch.uint8) if nb else None
+        _on(dev, lib.svk_gemm_i8, dt, pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), _p(bias), _p(residual), ldr,
+            out.data_ptr(), ldy, M, N, K, code, _p(ws), nb)
     return out

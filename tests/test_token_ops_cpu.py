@@ -84,10 +84,10 @@ def test_gated_ffn_bwd_workspace_covers_its_parts():
     for es, dt in ((2, 1), (2, 2), (4, 0)):
         for M, H, K in ((1, 1, 1), (100, 33, 64), (5000, 96, 61), (20000, 40, 72)):
             ld = (2 * H * es + 15) // 16 * 16
-            full = lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 1, 1)
+            full = lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 1, 1, 1)
             assert full >= M * ld + math.ceil(M / 64) * 2 * H * 4
-            assert lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 0, 0) <= full
-    assert lib.svk_gated_ffn_bwd_workspace(1, A, 8, A, 8, 0, 8, 8, 1, 1) == 0
+            assert lib.svk_gated_ffn_bwd_workspace(dt, A, K, A, K, M, H, K, 0, 0, 0) <= full
+    assert lib.svk_gated_ffn_bwd_workspace(1, A, 8, A, 8, 0, 8, 8, 1, 1, 1) == 0
 
 
 def _i8(lib, **kw):

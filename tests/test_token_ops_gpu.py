@@ -381,7 +381,8 @@ def test_gated_ffn_refusals(cuda):
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("M,K", [(1, 1), (5, 7), (3, 64), (130, 333), (9, 512), (4, 520), (2, 1024), (3, 2048), (2, 4096), (2, 5000), (2, 4099)])
 def test_quant_rows(cuda, dt, M, K):
-    """Scale and codes are f32 divisions, correctly rounded on both sides: equal bit for bit."""
+    """The scale and the factor 127 / max are f32 divisions, correctly rounded on both sides; their product with a value
+    is exact in 64 bits: equal bit for bit."""
     ops = _ops()
     x = _rand(M, K, dt=dt, seed=1, scale=3.0)
     if M > 1:
@@ -389,7 +390,8 @@ def test_quant_rows(cuda, dt, M, K):
     q, s = ops.quant_rows(x)
     xf = x.float().cpu()
     want_s = xf.abs().amax(1) / 127
-    want_q = torch.where(want_s[:, None] > 0, torch.round(xf / want_s[:, None]), torch.zeros_like(xf))
+    inv = torch.tensor(127.0) / xf.abs().amax(1, keepdim=True)       # (127 / tensor would be a reciprocal and a product)
+    want_q = torch.where(want_s[:, None] > 0, torch.round(xf.double() * inv.double()), torch.zeros_like(xf).double())
     assert q.shape == (M, K) and s.shape == (M,) and q.stride(0) % 16 == 0
     assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q.to(torch.int8))
     # a row's values are kept to half a step of its scale
