@@ -59,6 +59,11 @@ struct GateEpi {
   T* pre;                 // [M, 2H] contiguous, or null
   const float* bias;      // [2H] or null
   int M, H, act, per;
+  bool past;              // rows of h and pre are whole 16-byte pieces
+  void skip(long rows) {
+    h += rows * ldh;
+    if (pre) pre += rows * 2 * H;
+  }
 
   __device__ __forceinline__ float activate(float g) const { return glu_act<T>(g, ACT < 0 ? act : ACT); }
   // a wave's columns: half gate, half up rows of the same hidden channels; the pairs of blocks interleaved where each
@@ -90,6 +95,11 @@ struct GateEpi {
   }
   template <class C, typename A>
   __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int) const {
+    if (C::NONTEMPORAL && past) rows_of<C, true>(acc, m0, tn, wn, fq);
+    else rows_of<C, false>(acc, m0, tn, wn, fq);
+  }
+  template <class C, bool NTS, typename A>
+  __device__ __forceinline__ void rows_of(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
     constexpr int TG = C::TN / 2, W = width<C>(), S = W / 4;
     static_assert(C::TN % 2 == 0 && TG % S == 0, "a wave's columns are half gate, half up");
 #pragma unroll
@@ -115,10 +125,10 @@ struct GateEpi {
           o[e] = activate(g[e]) * u[e];
         }
         if (pre) {
-          put<T, W, C::NONTEMPORAL>(pre + (long)m * 2 * H + c, g, left);
-          put<T, W, C::NONTEMPORAL>(pre + (long)m * 2 * H + H + c, u, left);
+          put<T, W, NTS>(pre + (long)m * 2 * H + c, g, left);
+          put<T, W, NTS>(pre + (long)m * 2 * H + H + c, u, left);
         }
-        put<T, W, C::NONTEMPORAL>(h + (long)m * ldh + c, o, left);
+        put<T, W, NTS>(h + (long)m * ldh + c, o, left);
       }
     }
   }
@@ -130,8 +140,15 @@ struct PlainEpi {
   T* y; long ldy;
   float* slab;            // [parts][M][N], or null
   int M, N;
+  bool past;              // rows of y are whole 16-byte pieces
+  void skip(long rows) { y += rows * ldy; }      // never with slabs
   template <class C, typename A>
   __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int part) const {
+    if (C::NONTEMPORAL && past) rows_of<C, true>(acc, m0, tn, wn, fq, part);
+    else rows_of<C, false>(acc, m0, tn, wn, fq, part);
+  }
+  template <class C, bool NTS, typename A>
+  __device__ __forceinline__ void rows_of(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int part) const {
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
       const int n = tn * C::BN + wn * C::WN + j * 16 + fq * 4, left = N - n;
@@ -142,22 +159,68 @@ struct PlainEpi {
         if (m >= M) continue;
         const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
         if (slab) put<float, 4, false>(slab + ((long)part * M + m) * N + n, v, left);
-        else put<T, 4, C::NONTEMPORAL>(y + (long)m * ldy + n, v, left);
+        else put<T, 4, NTS>(y + (long)m * ldy + n, v, left);
       }
     }
   }
 };
 
-// y[m][n] = sum of the parts' slabs, in order
+// The joins of the backward pass, one launch: results whose reduction was split, y[m][n] = sum of the parts' f32 slabs in
+// order, and the bias gradient, db[c] = sum of the row blocks' sums.  Workgroups 0 .. first - 1 join x, then w, then the bias.
+struct Slabs {
+  const float* S;         // [parts][M][N]
+  void* y; long ldy;
+  int parts, M, N, blocks;        // workgroups that join it
+};
+constexpr int JOIN = 4;   // values a thread
 template <typename T>
-__global__ __launch_bounds__(256) void join_parts(const float* __restrict__ S, int parts, T* __restrict__ y, long ldy, int M,
-                                                  int N) {
-  const long total = (long)M * N;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    float v = 0.f;
-    for (int s = 0; s < parts; ++s) v += S[s * total + i];
-    const long m = i / N;
-    y[m * ldy + (i - m * N)] = from_f<T>(v);
+__device__ __forceinline__ void join_slabs(const Slabs& j, int block) {
+  const long total = (long)j.M * j.N;
+  T* y = static_cast<T*>(j.y);
+  for (long i = ((long)block * 256 + threadIdx.x) * JOIN; i < total; i += (long)j.blocks * 256 * JOIN) {
+    float v[JOIN] = {0.f, 0.f, 0.f, 0.f};
+    if (total % JOIN == 0) {
+      for (int s = 0; s < j.parts; ++s) {
+        const f32x4 p = *reinterpret_cast<const f32x4*>(j.S + s * total + i);
+#pragma unroll
+        for (int e = 0; e < JOIN; ++e) v[e] += p[e];
+      }
+    } else {
+      for (int s = 0; s < j.parts; ++s)
+#pragma unroll
+        for (int e = 0; e < JOIN; ++e)
+          if (i + e < total) v[e] += j.S[s * total + i + e];
+    }
+    const long m = i / j.N;
+    const int n = (int)(i - m * j.N);
+    if (n + JOIN <= j.N) put<T, JOIN, false>(y + m * j.ldy + n, v, JOIN);
+    else
+#pragma unroll
+      for (int e = 0; e < JOIN; ++e)
+        if (i + e < total) y[(i + e) / j.N * j.ldy + (i + e) % j.N] = from_f<T>(v[e]);
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void join_all(Slabs x, Slabs w, const float* __restrict__ S, int rows, float* __restrict__ db,
+                                                int N) {
+  int b = blockIdx.x;
+  if (b < x.blocks) return join_slabs<T>(x, b);
+  b -= x.blocks;
+  if (b < w.blocks) return join_slabs<T>(w, b);
+  b -= w.blocks;
+  // 16 columns a workgroup, 16 threads a column
+  __shared__ float part[16][17];
+  const int cl = threadIdx.x & 15, t = threadIdx.x >> 4, c = b * 16 + cl;
+  float v = 0.f;
+  if (c < N)
+    for (int r = t; r < rows; r += 16) v += S[(long)r * N + c];
+  part[t][cl] = v;
+  __syncthreads();
+  if (t == 0 && c < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += part[i][cl];
+    db[c] = s;
   }
 }
 
@@ -209,31 +272,14 @@ __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, con
   }
 }
 
-// db[c] = sum of the row blocks' sums, in order: 16 columns a workgroup, 16 threads a column
-__global__ __launch_bounds__(256) void join_bias(const float* __restrict__ S, int blocks, float* __restrict__ db, int N) {
-  __shared__ float part[16][17];
-  const int cl = threadIdx.x & 15, t = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
-  float v = 0.f;
-  if (c < N)
-    for (int b = t; b < blocks; b += 16) v += S[(long)b * N + c];
-  part[t][cl] = v;
-  __syncthreads();
-  if (t == 0 && c < N) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += part[i][cl];
-    db[c] = s;
-  }
-}
-
 // rows a workgroup of gated_dpre: 64, fewer where that leaves CUs idle (16: 4 a wave)
 inline int dpre_rows(long m, long h) { return m * h >= 1L << 23 ? 64 : 16; }
 
-// workspace of the backward pass: [dpre][x padded][w padded][bias partials][slabs of dx, then of dw]
+// workspace of the backward pass: [dpre][x padded][w padded][bias partials][slabs of dx][slabs of dW]
 struct BwdWs {
-  long ldd, dpre, x, w, sums, slabs, total;
+  long ldd, dpre, x, w, sums, xslabs, wslabs, total;
   int rows;
-  Plan px{2, 1}, pw{2, 1};
+  Plan px{2, 1, 0, 2}, pw{2, 1, 0, 2};
   BwdWs(long es, long M, long H, long K, bool padx, bool db, bool dx, bool dw) {
     auto plan = [&](long m, long n, long k) {
       return es == 4 ? plan_tiles<float>(m, n, stages<float>(k), 64) : plan_tiles<bf16>(m, n, stages<bf16>(k), 64);
@@ -247,8 +293,9 @@ struct BwdWs {
     sums = db ? up16((M + rows - 1) / rows * 2 * H * 4) : 0;
     if (dx) px = plan(M, K, 2 * H);
     if (dw) pw = plan(2 * H, K, M);
-    slabs = std::max(px.parts > 1 ? up16(px.parts * M * K * 4) : 0, pw.parts > 1 ? up16(pw.parts * 2 * H * K * 4) : 0);
-    total = dpre + x + w + sums + slabs;
+    xslabs = px.parts > 1 ? up16(px.parts * M * K * 4) : 0;
+    wslabs = pw.parts > 1 ? up16(pw.parts * 2 * H * K * 4) : 0;
+    total = dpre + x + w + sums + xslabs + wslabs;
   }
 };
 
@@ -300,10 +347,11 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
+    const bool past = al16(Hout) && ldh * es % 16 == 0 && H * es % 16 == 0 && al16(pre);
     Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(X, ldx, K, es) && rows_ok(W, ldw, K, es);
-      GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0};
+      GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0, past};
       return few_tokens<T, 2>(p, vec, H, epi, st, "gated_ffn_few");
     }
     char* at = (char*)ws;
@@ -323,10 +371,10 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     p.abytes = (M - 1) * p.lda + p.K * es;
     p.bbytes = (2 * H - 1) * p.ldb + p.K * es;
     p.nk = stages<T>(p.K);
-    const int tile = plan_tiles<T>(M, 2 * H, p.nk, 1).tile;
+    const Plan plan = plan_tiles<T>(M, 2 * H, p.nk, 1);
     auto run = [&](auto act_c) {
-      GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0};
-      return launch_plan<T, false, false>(tile, p, M, 2 * H, epi, st, "gated_ffn");
+      GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0, past};
+      return launch_plan<T, false, false>(plan, p, M, 2 * H, epi, st, "gated_ffn");
     };
     if (act == SVK_GLU_SILU) return run(std::integral_constant<int, SVK_GLU_SILU>{});
     if (act == SVK_GLU_GELU) return run(std::integral_constant<int, SVK_GLU_GELU>{});
@@ -362,16 +410,19 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
   if (M && (!ws || !al16(ws) || ws_bytes < need.total)) { set_error("svk_gated_ffn_bwd: workspace too small or misaligned"); return SVK_EINVAL; }
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
+    auto blocks_of = [](long values) { return (int)std::min<long>((values + 256 * JOIN - 1) / (256 * JOIN), 4096); };
+    Slabs jx{};
+    Slabs jw{};
+    const int db_blocks = db ? (int)((2 * H + 15) / 16) : 0;
+    auto join = [&](const float* sums, int rows) -> int {
+      const int all = jx.blocks + jw.blocks + db_blocks;
+      if (!all) return SVK_OK;
+      hipLaunchKernelGGL((join_all<T>), dim3((unsigned)all), dim3(256), 0, st, jx, jw, sums, rows, db, (int)(2 * H));
+      return check_launch("join_all");
+    };
     if (M == 0) {                                   // no tokens: the sums are empty
-      if (dW) {
-        hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((2 * H * K + 255) / 256, 8192)), dim3(256), 0, st, nullptr, 0, (T*)dW, K, (int)(2 * H), (int)K);
-        if (int rc = check_launch("join_parts")) return rc;
-      }
-      if (db) {
-        hipLaunchKernelGGL(join_bias, dim3((unsigned)((2 * H + 15) / 16)), dim3(256), 0, st, nullptr, 0, db, (int)(2 * H));
-        return check_launch("join_bias");
-      }
-      return SVK_OK;
+      if (dW) jw = Slabs{nullptr, dW, K, 0, (int)(2 * H), (int)K, blocks_of(2 * H * K)};
+      return join(nullptr, 0);
     }
     char* at = (char*)ws;
     T* D = (T*)at;
@@ -402,27 +453,23 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
                          (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
     }
     if (int rc = check_launch("gated_dpre")) return rc;
-    if (db) {
-      hipLaunchKernelGGL(join_bias, dim3((unsigned)((2 * H + 15) / 16)), dim3(256), 0, st, sums, rowblocks, db, (int)(2 * H));
-      if (int rc = check_launch("join_bias")) return rc;
-    }
-    // y [m, n], of parts joined where the output has few tiles
-    auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, const char* name) -> int {
+    // y [m, n]; where its reduction is split, the parts' slabs, joined below
+    auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, Slabs& j, const char* name) -> int {
       p.nk = stages<T>(p.K);
-      p.parts = plan.parts;
-      PlainEpi<T> epi{y, ldy, p.parts > 1 ? (float*)at : nullptr, (int)m, (int)n};
-      if (int rc = launch_plan<T, decltype(ac)::value, true>(plan.tile, p, m, n, epi, st, name)) return rc;
-      if (p.parts == 1) return SVK_OK;
-      hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)std::min<long>((m * n + 255) / 256, 8192)), dim3(256), 0, st,
-                         (float*)at, p.parts, y, ldy, (int)m, (int)n);
-      return check_launch("join_parts");
+      float* slabs = plan.parts > 1 ? (float*)at : nullptr;
+      PlainEpi<T> epi{y, ldy, slabs, (int)m, (int)n, al16(y) && ldy * es % 16 == 0 && n * es % 16 == 0};
+      if (slabs) {
+        j = Slabs{slabs, y, ldy, plan.parts, (int)m, (int)n, blocks_of(m * n)};
+        at += up16(plan.parts * m * n * 4);
+      }
+      return launch_plan<T, decltype(ac)::value, true>(plan, p, m, n, epi, st, name);
     };
     const long Db = M * need.ldd * es;
     // the padding of D is zero and rows of W past 2H read as zero, so dx's reduction runs over whole chunks
     if (dX)
-      if (int rc = product(std::false_type{}, need.px, Args{(const char*)D, Wr, need.ldd * es, ldwb, Db, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1}, (T*)dX, lddx, M, K, "gated_ffn_dx")) return rc;
+      if (int rc = product(std::false_type{}, need.px, Args{(const char*)D, Wr, need.ldd * es, ldwb, Db, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1}, (T*)dX, lddx, M, K, jx, "gated_ffn_dx")) return rc;
     if (dW)
-      return product(std::true_type{}, need.pw, Args{(const char*)D, Xr, need.ldd * es, ldxb, Db, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, 1}, (T*)dW, K, 2 * H, K, "gated_ffn_dw");
-    return SVK_OK;
+      if (int rc = product(std::true_type{}, need.pw, Args{(const char*)D, Xr, need.ldd * es, ldxb, Db, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, 1}, (T*)dW, K, 2 * H, K, jw, "gated_ffn_dw")) return rc;
+    return join(sums, rowblocks);
   });
 }

@@ -4,7 +4,7 @@
 //   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] * (127 / max))      (ties to even; a row of zeros: s = 0, q = 0)
 //   C[m, n] = act((sum_k qa[m, k] qw[n, k]) sa[m] sw[n] + bias[n]) + R[m, n]
 //
-// The integer sums are exact (int32: K <= 131072 for codes of -128 .. 127); everything behind them is f32, rounded once.
+// The integer sums are exact (int32: K <= 131071, 2^31 / 128^2 less one); everything behind them is f32, rounded once.
 // A row with an infinity or a NaN gets the scale NaN and codes of zero: its outputs are NaN, not quietly wrong.
 // tile_mm.h with int8 operands: mfma 16x16x64 at twice the 16-bit rate and half the bytes.
 #include "tile_mm.h"
@@ -147,6 +147,12 @@ struct ScaleEpi {
   const T* R; long ldr;
   T* y; long ldy;
   int M, N, act, per;
+  bool past;              // rows of y are whole 16-byte pieces
+  void skip(long rows) {
+    sa += rows;
+    if (R) R += rows * ldr;
+    y += rows * ldy;
+  }
 
   __device__ __forceinline__ float value(int acc, float a, float w, float b) const {
     const float v = (float)acc * a * w + b;
@@ -167,6 +173,11 @@ struct ScaleEpi {
   }
   template <class C, typename A>
   __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int) const {
+    if (C::NONTEMPORAL && past) rows_of<C, true>(acc, m0, tn, wn, fq);
+    else rows_of<C, false>(acc, m0, tn, wn, fq);
+  }
+  template <class C, bool NTS, typename A>
+  __device__ __forceinline__ void rows_of(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq) const {
     constexpr int NW = 8 * sizeof(T) / 4;
     typedef uint32_t vec __attribute__((ext_vector_type(NW)));
     typedef vec anywhere __attribute__((aligned(2)));
@@ -216,7 +227,7 @@ struct ScaleEpi {
             v[e] = value(acc[i][j + e / 4][e % 4], a[i], w[e], b[e]);
             if (R) v[e] += to_f(t[e]);
           }
-          if (m < M) put<T, 8, C::NONTEMPORAL>(y + (long)m * ldy + n, v, left);
+          if (m < M) put<T, 8, NTS>(y + (long)m * ldy + n, v, left);
           __builtin_amdgcn_sched_barrier(0);                    // one row at a time: fewer registers
         }
       }
@@ -226,7 +237,7 @@ struct ScaleEpi {
 
 static bool rows_ok(const void* p, long ld, long K) { return al16(p) && ld % 16 == 0 && K % 16 == 0; }
 static bool bad_dims(long M, long N, long K) {
-  return M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00L || N > 0x7fffff00L || K > 131072;
+  return M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00L || N > 0x7fffff00L || K > 131071;
 }
 
 }  // namespace i8
@@ -275,7 +286,7 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
                            void* ws, long ws_bytes, void* stream) {
   if (!A || !sa || !W || !sw || !Y || bad_dims(M, N, K) || lda < K || ldw < K || ldy < N || (R && ldr < N) ||
       act < SVK_ACT_NONE || act > SVK_ACT_TANH) {
-    set_error("svk_gemm_i8: bad args (K up to 131072)");
+    set_error("svk_gemm_i8: bad args (K up to 131071)");
     return SVK_EINVAL;
   }
   const long ldk = up16(K);
@@ -287,10 +298,11 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
+    const bool past = al16(Y) && ldy * (long)sizeof(T) % 16 == 0 && N * (long)sizeof(T) % 16 == 0;
     Args p{(const char*)A, (const char*)W, lda, ldw, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       const bool vec = rows_ok(A, lda, K) && rows_ok(W, ldw, K);
-      ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0};
+      ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0, past};
       return few_tokens<int8_t, 1>(p, vec, N, epi, st, "gemm_i8_few");
     }
     char* at = (char*)ws;
@@ -315,10 +327,10 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
     p.nk = stages<int8_t>(p.K);
     p.abytes = (M - 1) * p.lda + p.K;
     p.bbytes = (N - 1) * p.ldb + p.K;
-    const int tile = plan_tiles<int8_t>(M, N, p.nk, 1).tile;
+    const Plan plan = plan_tiles<int8_t>(M, N, p.nk, 1);
     auto run = [&](auto act_c) {
-      ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0};
-      return launch_plan<int8_t, false, false>(tile, p, M, N, epi, st, "gemm_i8");
+      ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0, past};
+      return launch_plan<int8_t, false, false>(plan, p, M, N, epi, st, "gemm_i8");
     };
     if (act == SVK_ACT_NONE) return run(std::integral_constant<int, SVK_ACT_NONE>{});
     if (act == SVK_ACT_GELU) return run(std::integral_constant<int, SVK_ACT_GELU>{});

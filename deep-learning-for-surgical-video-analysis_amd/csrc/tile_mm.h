@@ -53,9 +53,8 @@ __device__ __forceinline__ i32x4 descriptor(const char* base, long left) {
 }
 // 16 bytes a lane from the descriptor's base + voff to LDS lds + 16 * lane
 __device__ __forceinline__ void dma16(i32x4 r, uint32_t voff, uint32_t lds) {
-  uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(voff), "s"(r), "s"(lds) : "memory");
+  // (m0 is told as clobbered rather than kept and put back: two scalar instructions a piece, 1.2 % of a large product)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "s"(lds) : "memory", "m0");
 }
 
 template <typename T> struct Acc { typedef f32x4 t; };
@@ -116,7 +115,8 @@ __device__ __forceinline__ void tile_of(int bid, int ntm, int ntn, int& tm, int&
   tn = in / g;
 }
 
-// W consecutive values of a row: one store (of any alignment) where all W exist, else one by one
+// W consecutive values of a row: one store (of any alignment) where all W exist, else one by one.  NTS: past the L2;
+// only for rows of whole 16-byte pieces (partial lines past the L2 cost: 50176 x 320 x 2 x 853 in f16 107 us, 99 without)
 template <typename T, int W, bool NTS>
 __device__ __forceinline__ void put(T* at, const float* v, int n) {
   T o[W];
@@ -156,6 +156,7 @@ __device__ __forceinline__ float gelu16(float x) {
 // Epi (row operand B): uint32_t offset<C>(r, ldb): bytes from the tile's first row to B row r of the tile;
 //                      long first<C>(tn): the tile's first row
 //      write<C>(acc, m, tn, wn, fq, part): stores the tile; acc[i][j]: row m + 16 i, columns 4 fq .. of block j
+//      M: its rows;  skip(rows): begins that many rows later
 template <typename T, class C, bool ACOL, bool BCOL, class Epi>
 __global__ __launch_bounds__(C::NT, C::OCC) void tile_mm(Args p, Epi epi) {
   constexpr int ES = sizeof(T), BK = 128 / ES;
@@ -347,7 +348,9 @@ using Small = Tile<64, 64, 2, 2, 3, 3>;        // three
 // less than `alone` us; `end` us a tile for its results.  Measured on 1 to 50176 rows, 96 to 5632 results, 64 to 2048
 // values of k; the choice is the best of the three, or within 10 % of it, at nearly all of them (1500 x 1024 x 2 x 5632
 // in bf16: 128-wide 50, 256-wide 57, 64-wide 68 us; 6000 x 2048 x 2 x 1024: 60, 51, 95; 100 x 2048 x 2 x 340: 24, 45, 14).
-struct Plan { int tile, parts; };
+// Where the last round of tiles would leave most CUs idle, the rows behind the whole rounds are taken by a second launch
+// with smaller tiles (352 tiles of 256 for 256 CUs: 404 -> DWT us).
+struct Plan { int tile, parts; long rows; int rest; };          // the first `rows` rows with `tile`, the others with `rest`
 struct Rate { double alone, step, end; };
 template <typename T>
 inline Plan plan_tiles(long m, long n, long nk, long most) {
@@ -355,19 +358,32 @@ inline Plan plan_tiles(long m, long n, long nk, long most) {
   constexpr Rate r8[3] = {{1.1, 1.5, 8.0}, {0.5, 0.45, 2.2}, {0.21, 0.2, 0.7}};
   constexpr Rate r32[3] = {{7.3, 7.3, 4.0}, {2.1, 2.0, 1.3}, {0.72, 0.54, 0.5}};
   const Rate* rates = sizeof(T) == 4 ? r32 : (sizeof(T) == 1 ? r8 : r16);
-  Plan best{2, 1};
+  auto cost = [&](int c, long rows, long parts, long per) {
+    const long side = 256 >> c;
+    const double tiles = (double)((rows + side - 1) / side) * (double)((n + side - 1) / side);
+    const double each = ceil(tiles * (double)parts / 256.0);
+    return (double)per * fmax(rates[c].alone, each * rates[c].step) + each * rates[c].end;
+  };
+  Plan best{2, 1, m, 2};
   double least = 1e30;
   for (int c = 0; c < 3; ++c) {
-    const long side = 256 >> c;
-    const double tiles = (double)((m + side - 1) / side) * (double)((n + side - 1) / side);
     for (long parts = 1; parts <= most && (parts == 1 || nk >= 4 * parts); parts *= 2) {
       const long per = (nk + parts - 1) / parts, real = (nk + per - 1) / per;      // no empty part
-      const double each = ceil(tiles * (double)real / 256.0), k = (double)per;
-      double t = k * fmax(rates[c].alone, each * rates[c].step) + each * rates[c].end;
+      double t = cost(c, m, real, per);
       if (real > 1) t += 4.0 + (double)m * (double)n * 4.0 * (double)(real + 1) / 4e6;        // the slabs and their join
       if (t < least) {
         least = t;
-        best = Plan{c, (int)real};
+        best = Plan{c, (int)real, m, c};
+      }
+    }
+    const long side = 256 >> c, ntn = (n + side - 1) / side, rounds = (m + side - 1) / side * ntn / 256;
+    const long rows = rounds * 256 / ntn * side;                // rows of the whole rounds
+    if (rows <= 0 || rows >= m) continue;
+    for (int d = c + 1; d < 3; ++d) {
+      const double t = cost(c, rows, 1, nk) + 3.0 + cost(d, m - rows, 1, nk);
+      if (t < least) {
+        least = t;
+        best = Plan{c, 1, rows, d};
       }
     }
   }
@@ -402,10 +418,24 @@ static int launch_tiles(Args p, long m, long n, const Epi& epi, hipStream_t st, 
   return check_launch(name);
 }
 template <typename T, bool AC, bool BC, class Epi>
-static int launch_plan(int tile, const Args& p, long m, long n, const Epi& epi, hipStream_t st, const char* name) {
-  if (tile == 0) return launch_tiles<T, Big, AC, BC>(p, m, n, epi, st, name);
-  if (tile == 1) return launch_tiles<T, Mid, AC, BC>(p, m, n, epi, st, name);
-  return launch_tiles<T, Small, AC, BC>(p, m, n, epi, st, name);
+static int launch_plan(const Plan& plan, Args p, long m, long n, Epi epi, hipStream_t st, const char* name) {
+  auto go = [&](int tile, long rows) -> int {
+    if (tile == 0) return launch_tiles<T, Big, AC, BC>(p, rows, n, epi, st, name);
+    if (tile == 1) return launch_tiles<T, Mid, AC, BC>(p, rows, n, epi, st, name);
+    return launch_tiles<T, Small, AC, BC>(p, rows, n, epi, st, name);
+  };
+  p.parts = plan.parts;
+  const long last = epi.M;
+  epi.M = (int)plan.rows;
+  if (int rc = go(plan.tile, plan.rows)) return rc;
+  if (plan.rows >= m) return SVK_OK;
+  // the rest: the operand and the results from row plan.rows on
+  const long skip = AC ? plan.rows * (long)sizeof(T) : plan.rows * p.lda;
+  p.A += skip;
+  p.abytes -= skip;
+  epi.M = (int)(last - plan.rows);
+  epi.skip(plan.rows);
+  return go(plan.rest, m - plan.rows);
 }
 template <typename T> inline int stages(long k) { return (int)((k * (long)sizeof(T) + 127) / 128); }
 

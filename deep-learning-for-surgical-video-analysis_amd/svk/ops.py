@@ -1483,6 +1483,7 @@ def mstcn_bwd_floats(T, F):
 
 GLU_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 _POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_FEW = 64          # tokens up to which the few-token kernels run: they read rows of any alignment and take no workspace
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch.cuda.current_device
 
@@ -1703,7 +1704,7 @@ def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
     pre = torch.empty((*lead, 2 * H), device=x.device, dtype=x.dtype) if save else None
     if M:
         lib, px, pw = _lib.load(), x.data_ptr(), w.data_ptr()
-        nb = lib.svk_gated_ffn_workspace(dt, px, ldx, pw, ldw, M, H, K)
+        nb = 0 if M <= _FEW else lib.svk_gated_ffn_workspace(dt, px, ldx, pw, ldw, M, H, K)
         ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
         _on(dev, lib.svk_gated_ffn, dt, px, ldx, pw, ldw, _p(bias), out.data_ptr(), ldh, _p(pre), M, H, K, code, _p(ws), nb)
     return (out, pre) if save else out
@@ -1757,7 +1758,7 @@ def quant_rows(x):
 def gemm_i8(a, a_scale, w, w_scale, bias=None, act=None, residual=None, out=None, dtype=torch.float16):
     """act((a @ w.T as exact integers) * a_scale[m] * w_scale[n] + bias) + residual (svk_gemm_i8): a int8 [..., K] with
     a_scale float32 [...], w int8 [N, K] with w_scale float32 [N] (both from quant_rows) -> [..., N] in ``dtype`` (or
-    out's).  K <= 131072.  ``out`` may be ``residual``."""
+    out's).  K <= 131071.  ``out`` may be ``residual``."""
     fn = "gemm_i8"
     dev = a.get_device()
     if dev < 0:
@@ -1799,7 +1800,7 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, act=None, residual=None, out=None
         _, _, ldr = _token_rows(residual, fn, "residual")
     if M:
         lib, pa, pw = _lib.load(), a.data_ptr(), w.data_ptr()
-        nb = lib.svk_gemm_i8_workspace(pa, lda, pw, ldw, M, N, K)
+        nb = 0 if M <= _FEW else lib.svk_gemm_i8_workspace(pa, lda, pw, ldw, M, N, K)
         ws = torch.empty(nb, device=a.device, dtype=torch.uint8) if nb else None
         _on(dev, lib.svk_gemm_i8, dt, pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), _p(bias), _p(residual), ldr,
             out.data_ptr(), ldy, M, N, K, code, _p(ws), nb)

@@ -61,7 +61,10 @@ def test_gated_ffn_sizes():
     assert ws(1, A, 64, A, 64, 100, 32, 64) == 0
     assert ws(1, A, 63, A, 63, 100, 32, 63) == (100 + 64) * 128      # both padded to 128-byte rows
     assert ws(1, A + 2, 64, A, 64, 100, 32, 64) == 100 * 128         # x misaligned
-    assert ws(1, A, 63, A, 63, 8, 32, 63) == 0                       # few tokens: read as they are
+    from svk import ops
+    for M, want in ((8, 0), (ops._FEW, 0), (ops._FEW + 1, (ops._FEW + 65) * 128)):      # few tokens: read as they are
+        assert ws(1, A, 63, A, 63, M, 32, 63) == want
+        assert (lib.svk_gemm_i8_workspace(A, 63, A, 63, M, 64, 63) == 0) == (want == 0)
 
 
 def _gated_bwd(lib, **kw):
@@ -99,7 +102,7 @@ def _i8(lib, **kw):
 
 @pytest.mark.parametrize("kw", [dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None), dict(lda=63),
                                 dict(ldw=63), dict(ldy=47), dict(R=A, ldr=47), dict(M=-1), dict(N=0), dict(K=0),
-                                dict(K=131073, lda=131073, ldw=131073), dict(act=4), dict(act=-1),
+                                dict(K=131072, lda=131072, ldw=131072), dict(act=4), dict(act=-1),
                                 dict(lda=65)])                        # the last: rows to be padded, no workspace
 def test_gemm_i8_refuses(kw):
     lib = _lib()

@@ -454,12 +454,14 @@ def test_gemm_i8_large_tiles_exact(cuda, M, N, K):
 def test_gemm_i8_exact_sums_views_and_extremes(cuda):
     ops = _ops()
     one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
-    for M in (2, 40):
-        # the longest reduction at the largest codes: 131072 * 127 * 127 in int32
-        a = torch.full((M, 131072), 127, dtype=torch.int8, device="cuda")
-        w = torch.full((3, 131072), -127, dtype=torch.int8, device="cuda")
+    for M in (2, 70):
+        # the longest reduction at the largest codes: 131071 * 128 * 128 = 2^31 - 2^14 in int32
+        a = torch.full((M, 131071), -128, dtype=torch.int8, device="cuda")
+        w = torch.full((3, 131071), -128, dtype=torch.int8, device="cuda")
+        w[1] = 127
         got = ops.gemm_i8(a, one(M), w, one(3), dtype=torch.float32)
-        assert torch.equal(got, torch.full((M, 3), -127.0 * 127 * 131072, device="cuda"))
+        want = torch.tensor([128.0 * 128 * 131071, -128.0 * 127 * 131071, 128.0 * 128 * 131071], device="cuda")
+        assert torch.equal(got, want.expand(M, 3))
         ab, wb = _codes(M, 90, 3), _codes(20, 90, 4)
         for x, y in ((ab[:, 16:80], wb[:, 16:80]), (ab[:, 1:60], wb[:, 2:61])):
             out = torch.full((M + 2, 26), 9.0, device="cuda")
@@ -493,8 +495,8 @@ def test_i8_refusals(cuda):
                dict(a_scale=sa.half()), dict(bias=sw[:5]), dict(residual=r[:3]), dict(residual=r.float()), dict(act="silu"),
                dict(dtype=torch.float64), dict(dtype=torch.int8), dict(out=r[:3]), dict(a=a.t()), dict(w=w[:0]), dict(w=w.cpu()),
                dict(out=r.double()), dict(w_scale=torch.ones(12, device="cuda")[::2]), dict(a=a.cpu()),
-               dict(a=torch.zeros(2, 131073, dtype=torch.int8, device="cuda"), a_scale=sa[:2],
-                    w=torch.zeros(6, 131073, dtype=torch.int8, device="cuda")),
+               dict(a=torch.zeros(2, 131072, dtype=torch.int8, device="cuda"), a_scale=sa[:2],
+                    w=torch.zeros(6, 131072, dtype=torch.int8, device="cuda")),
                dict(out=torch.zeros(1, 6, device="cuda").expand(4, 6)), dict(residual=r, out=r.flatten()[:24].view(6, 4).t())):
         with pytest.raises(svk.SvkError):
             f(**kw)
