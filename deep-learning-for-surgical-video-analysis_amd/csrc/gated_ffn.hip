@@ -166,7 +166,7 @@ struct PlainEpi {
 };
 
 // The joins of the backward pass, one launch: results whose reduction was split, y[m][n] = sum of the parts' f32 slabs in
-// order, and the bias gradient, db[c] = sum of the row blocks' sums.  Workgroups 0 .. first - 1 join x, then w, then the bias.
+// order, and the bias gradient, db[c] = sum of the row blocks' sums.  The first workgroups join dx, then come dW's, then the bias's.
 struct Slabs {
   const float* S;         // [parts][M][N]
   void* y; long ldy;

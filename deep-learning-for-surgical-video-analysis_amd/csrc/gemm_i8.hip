@@ -33,7 +33,8 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // The largest magnitude is found on the bits without the sign, whose order as integers is that of the magnitudes (an
 // infinity or a NaN comes out largest).  A code is the product with 127 / max and 1.5 * 2^23 added in one fma: the sum's
 // last byte is the nearest integer to the exact product, ties to even.  (Three instructions a value; a division, a
-// rounding and two clamps each took 12544 rows of 512 f16 11.0 us, and this QRN.)
+// rounding and two clamps each, and one row a wave, took 12544 rows of 512 in f16 11.0 us, this 8.9; 16384 rows of 4096 in
+// bf16 46 and 33 us: 201 MB at 6.1 TB/s.)
 template <typename T, int NCH, int RW, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long ldx, int8_t* __restrict__ Q, long ldq,
                                                   float* __restrict__ S, long M, int K) {
