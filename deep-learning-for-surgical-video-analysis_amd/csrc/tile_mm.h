@@ -150,7 +150,8 @@ __device__ __forceinline__ float gelu16(float x) {
   q = fmaf(q, t, s * -0.284496736f);
   q = fmaf(q, t, s * 0.254829592f);
   const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);                // -x^2 / 2 * log2(e)
-  return fmaf(fminf(fabsf(x), 1e4f) * t * q, e, x > 0.f ? x : 0.f);                     // bounded: infinity times t = 0
+  // medians: |x| bounded (infinity times t = 0 is no number), and x where it is positive; one instruction each
+  return fmaf(__builtin_amdgcn_fmed3f(fabsf(x), 0.f, 1e4f) * t * q, e, __builtin_amdgcn_fmed3f(x, 0.f, INFINITY));
 }
 
 // Epi (row operand B): uint32_t offset<C>(r, ldb): bytes from the tile's first row to B row r of the tile;
