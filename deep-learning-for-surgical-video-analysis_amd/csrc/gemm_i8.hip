@@ -1,7 +1,7 @@
 // Matrix product in 8-bit integers with a scale for each token and each output channel (svk_gemm_i8), and the
 // quantisation of token rows that feeds it (svk_quant_rows):
 //
-//   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] * (127 / max))      (ties to even; a row of zeros: s = 0, q = 0)
+//   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] / s[m])            (ties to even; a row of zeros: s = 0, q = 0)
 //   C[m, n] = act((sum_k qa[m, k] qw[n, k]) sa[m] sw[n] + bias[n]) + R[m, n]
 //
 // The integer sums are exact (int32: K <= 131071, 2^31 / 128^2 less one); everything behind them is f32, rounded once.
@@ -31,10 +31,12 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // RW rows a wave, read before the first is reduced; NCH chunks of 8 values a lane and row kept in registers (0: read
 // twice).
 // The largest magnitude is found on the bits without the sign, whose order as integers is that of the magnitudes (an
-// infinity or a NaN comes out largest).  A code is the product with 127 / max and 1.5 * 2^23 added in one fma: the sum's
-// last byte is the nearest integer to the exact product, ties to even.  (Three instructions a value; a division, a
-// rounding and two clamps each, and one row a wave, took 12544 rows of 512 in f16 11.0 us, this 8.9; 16384 rows of 4096 in
-// bf16 46 and 33 us: 201 MB at 6.1 TB/s.)
+// infinity or a NaN comes out largest).  A code is the correctly rounded quotient x / s, rounded to an integer: with r the
+// correctly rounded 1 / s and y = x r, the residual x - y s is exact in one fma, and y + residual * r is the correctly
+// rounded quotient (Markstein); 1.5 * 2^23 added to it leaves the nearest integer, ties to even, in the last byte.  Four
+// instructions a value; the division, a rounding and two clamps each, and one row a wave, took 12544 rows of 512 in f16
+// 11.0 us, this 9.6; 16384 rows of 4096 in bf16 46 and 33 us (201 MB at 6.1 TB/s).  (x * (127 / max) would take one, but decides the
+// many exact ties of 16-bit values another way than x / s.)
 template <typename T, int NCH, int RW, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long ldx, int8_t* __restrict__ Q, long ldq,
                                                   float* __restrict__ S, long M, int K) {
@@ -43,16 +45,18 @@ __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long 
   if (row0 >= M) return;
   constexpr int W = 2 * sizeof(T);                              // words of 8 values
   float s, inv;
-  // the scale from the largest magnitude; inv = 127 / max, or 0 where that is no finite number: then codes come from a
-  // division (rows of subnormal values) or are 0
+  // the scale from the largest magnitude, and its reciprocal; 0 where the scale is so small that the residual would
+  // underflow (then codes come from the division), or is no finite number, or 0 (codes of 0)
   auto scale = [&](long row, float top) {
     s = top < INFINITY ? top / 127.f : NAN;
-    inv = 127.f / top;
-    if (!(inv < INFINITY) || !(top < INFINITY)) inv = 0.f;
+    inv = s >= 1e-30f ? 1.f / s : 0.f;
     if (lane == 0) S[row] = s;
   };
   auto code = [&](float v) -> uint32_t {
-    if (inv > 0.f) return __float_as_uint(fmaf(v, inv, 12582912.f)) & 255u;
+    if (inv > 0.f) {
+      const float y = v * inv;
+      return __float_as_uint(fmaf(fmaf(-y, s, v), inv, y) + 12582912.f) & 255u;
+    }
     if (s > 0.f) return (uint32_t)(int)rintf(fminf(fmaxf(v / s, -127.f), 127.f)) & 255u;
     return 0u;
   };

@@ -381,8 +381,7 @@ def test_gated_ffn_refusals(cuda):
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("M,K", [(1, 1), (5, 7), (3, 64), (130, 333), (9, 512), (4, 520), (2, 1024), (3, 2048), (2, 4096), (2, 5000), (2, 4099)])
 def test_quant_rows(cuda, dt, M, K):
-    """The scale and the factor 127 / max are f32 divisions, correctly rounded on both sides; their product with a value
-    is exact in 64 bits: equal bit for bit."""
+    """The scale and x / scale are f32 divisions, correctly rounded on both sides: equal bit for bit."""
     ops = _ops()
     x = _rand(M, K, dt=dt, seed=1, scale=3.0)
     if M > 1:
@@ -390,12 +389,33 @@ def test_quant_rows(cuda, dt, M, K):
     q, s = ops.quant_rows(x)
     xf = x.float().cpu()
     want_s = xf.abs().amax(1) / 127
-    inv = torch.tensor(127.0) / xf.abs().amax(1, keepdim=True)       # (127 / tensor would be a reciprocal and a product)
-    want_q = torch.where(want_s[:, None] > 0, torch.round(xf.double() * inv.double()), torch.zeros_like(xf).double())
+    want_q = torch.where(want_s[:, None] > 0, torch.round(xf / want_s[:, None]), torch.zeros_like(xf))
     assert q.shape == (M, K) and s.shape == (M,) and q.stride(0) % 16 == 0
     assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q.to(torch.int8))
     # a row's values are kept to half a step of its scale
     _within(q.to(F64) * s.to(F64)[:, None], x.to(F64), (0.5 + 2.0 ** -15) * s.to(F64)[:, None].expand(M, K) + 1e-30, "values")
+
+
+def test_quant_rows_ties_and_scales_of_all_sizes(cuda):
+    """Quotients on and next to half integers (16-bit values divide to exact ties often), and scales from subnormal to
+    1e36: still the correctly rounded quotient, rounded."""
+    ops = _ops()
+    n = torch.arange(-127, 128, dtype=torch.float32) * 0.5
+    x = torch.cat([n, torch.nextafter(n, n + 1), torch.nextafter(n, n - 1), torch.tensor([127.0, 126.99999])])
+    g = torch.Generator().manual_seed(5)
+    rows = [x * 2.0 ** e * f for e in (-140, -126, -100, -60, 0, 60, 110) for f in (1.0, 1.1, 1.9999999)]
+    rows += [torch.randn(len(x), generator=g).half().float() * 2.0 ** -e for e in range(12)]
+    x = torch.stack(rows)
+    s = x.abs().amax(1, keepdim=True) / 127
+    want = torch.where(s > 0, torch.round(x / s), torch.zeros_like(x)).clamp(-127, 127)
+    q, sc = ops.quant_rows(x.cuda())
+    fine = s[:, 0] >= 2.0 ** -126                 # a subnormal scale is a rough number, but the same on both sides
+    assert torch.equal(sc.cpu()[fine], s[fine, 0]) and torch.equal(q.cpu()[fine].float(), want[fine])
+    assert int(q.abs().max()) <= 127
+    for dt in (torch.float16, torch.bfloat16):
+        y = (torch.randint(-2000, 2001, (500, 256), generator=g).float() / 64).to(dt)
+        s = y.float().abs().amax(1, keepdim=True) / 127
+        assert torch.equal(ops.quant_rows(y.cuda())[0].cpu().float(), torch.round(y.float() / s))
 
 
 def test_quant_rows_not_finite_tiny_and_views(cuda):
