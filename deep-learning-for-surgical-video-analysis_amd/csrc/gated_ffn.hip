@@ -226,22 +226,37 @@ __global__ __launch_bounds__(256) void join_all(Slabs x, Slabs w, const float* _
 
 // dg, du from the kept projections: D [M][ld] = dg | du | zeros up to ld; S [row blocks][2H] = their column sums over
 // a block of rows, f32, before the rounding.  4 waves a workgroup, 64 * V columns, rows dealt to the waves in turn.
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, const T* __restrict__ dh, long lddh,
                                                   T* __restrict__ D, long ld, float* __restrict__ S, int M, int H, int act, int rows) {
+  constexpr int V = 16 / (int)sizeof(T);
   __shared__ float sum[2][4][64 * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (blockIdx.y * 64 + lane) * V;
   const long r0 = (long)blockIdx.x * rows, r1 = min(r0 + rows, (long)M);
-  const int nc = H - c;                       // columns that exist from c on (V divides H where V > 1)
+  const int nc = H - c;                       // columns that exist from c on
   float sg[V], su[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sg[e] = su[e] = 0.f;
   typedef T vec __attribute__((ext_vector_type(V)));
+  typedef vec anywhere __attribute__((aligned(sizeof(T))));
+  auto get = [&](const T* p) -> vec {         // V columns at any alignment, zeros past the last
+    if (nc >= V) return *reinterpret_cast<const anywhere*>(p);
+    vec v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < nc ? p[e] : from_f<T>(0.f);
+    return v;
+  };
+  auto set = [&](T* p, const vec& v) {
+    if (nc >= V) *reinterpret_cast<anywhere*>(p) = v;
+    else
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < nc) p[e] = v[e];
+  };
   for (long r = r0 + wave; r < r1; r += 4) {
     if (nc > 0) {
-      const vec g = *reinterpret_cast<const vec*>(pre + r * 2 * H + c), u = *reinterpret_cast<const vec*>(pre + r * 2 * H + H + c);
-      const vec d = *reinterpret_cast<const vec*>(dh + r * lddh + c);
+      const vec g = get(pre + r * 2 * H + c), u = get(pre + r * 2 * H + H + c), d = get(dh + r * lddh + c);
       vec og, ou;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -253,8 +268,8 @@ __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, con
         sg[e] += dg;
         su[e] += du;
       }
-      *reinterpret_cast<vec*>(D + r * ld + c) = og;
-      *reinterpret_cast<vec*>(D + r * ld + H + c) = ou;
+      set(D + r * ld + c, og);
+      set(D + r * ld + H + c, ou);
     }
     // the padding of the row, by the last column block
     if (blockIdx.y == gridDim.y - 1 && 2 * H + lane < ld) D[r * ld + 2 * H + lane] = from_f<T>(0.f);
@@ -304,14 +319,6 @@ static bool bad_dims(long M, long H, long K) {
   return M < 0 || H <= 0 || K <= 0 || M > 0x7fffff00L || H > 4000000L || K > 0x1fffff00L;
 }
 
-template <typename T>
-static int pad(const void* X, long ldx, void* Y, long rows, long K, hipStream_t st) {
-  const long ld = up16(K * (long)sizeof(T)) / (long)sizeof(T);
-  const long blocks = std::min<long>((rows * ld + 255) / 256, 8192);
-  hipLaunchKernelGGL((pad_rows<T>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)X, ldx, (T*)Y, ld, rows, (int)K);
-  return check_launch("pad_rows");
-}
-
 static int es_of(int dtype) { return dtype == SVK_F32 ? 4 : (dtype == SVK_BF16 || dtype == SVK_F16 ? 2 : 0); }
 
 }  // namespace gf
@@ -350,20 +357,19 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     const bool past = al16(Hout) && ldh * es % 16 == 0 && H * es % 16 == 0 && al16(pre);
     Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
-      const bool vec = rows_ok(X, ldx, K, es) && rows_ok(W, ldw, K, es);
       GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0, past};
-      return few_tokens<T, 2>(p, vec, H, epi, st, "gated_ffn_few");
+      return few_tokens<T, 2>(p, H, epi, st, "gated_ffn_few");
     }
     char* at = (char*)ws;
     if (!rows_ok(X, ldx, K, es)) {
-      if (int rc = pad<T>(X, ldx, at, M, K, st)) return rc;
+      if (int rc = pad<T>(X, ldx * es, at, M, K * es, st)) return rc;
       p.A = at;
       p.lda = ldk;
       at += M * ldk;
       p.K = (int)(ldk / es);
     }
     if (!rows_ok(W, ldw, K, es)) {
-      if (int rc = pad<T>(W, ldw, at, 2 * H, K, st)) return rc;
+      if (int rc = pad<T>(W, ldw * es, at, 2 * H, K * es, st)) return rc;
       p.B = at;
       p.ldb = ldk;
       p.K = (int)(ldk / es);
@@ -431,11 +437,11 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     long ldxb = ldx * es, ldwb = ldw * es;
     const long kb = padx ? ldk : K * es;            // bytes of a row of either
     if (padx) {
-      if (int rc = pad<T>(X, ldx, at, M, K, st)) return rc;
+      if (int rc = pad<T>(X, ldx * es, at, M, K * es, st)) return rc;
       Xr = at;
       ldxb = ldk;
       at += need.x;
-      if (int rc = pad<T>(W, ldw, at, 2 * H, K, st)) return rc;
+      if (int rc = pad<T>(W, ldw * es, at, 2 * H, K * es, st)) return rc;
       Wr = at;
       ldwb = ldk;
       at += need.w;
@@ -444,14 +450,8 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     at += need.sums;
     const int rowblocks = (int)((M + need.rows - 1) / need.rows);
     constexpr int V = 16 / (int)sizeof(T);
-    auto al = [&](const void* q) { return ((uintptr_t)q & 15) == 0; };
-    if (H % V == 0 && lddh % V == 0 && al(pre) && al(dH)) {
-      hipLaunchKernelGGL((gated_dpre<T, V>), dim3(rowblocks, (unsigned)((H + 64 * V - 1) / (64 * V))), dim3(256), 0, st,
-                         (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
-    } else {
-      hipLaunchKernelGGL((gated_dpre<T, 1>), dim3(rowblocks, (unsigned)((H + 63) / 64)), dim3(256), 0, st, (const T*)pre,
-                         (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
-    }
+    hipLaunchKernelGGL((gated_dpre<T>), dim3(rowblocks, (unsigned)((H + 64 * V - 1) / (64 * V))), dim3(256), 0, st,
+                       (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
     if (int rc = check_launch("gated_dpre")) return rc;
     // y [m, n]; where its reduction is split, the parts' slabs, joined below
     auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, Slabs& j, const char* name) -> int {

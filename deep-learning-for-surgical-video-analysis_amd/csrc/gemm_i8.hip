@@ -37,7 +37,7 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // instructions a value; the division, a rounding and two clamps each, and one row a wave, took 12544 rows of 512 in f16
 // 11.0 us, this 9.6; 16384 rows of 4096 in bf16 46 and 33 us (201 MB at 6.1 TB/s).  (x * (127 / max) would take one, but decides the
 // many exact ties of 16-bit values another way than x / s.)
-template <typename T, int NCH, int RW, bool VEC>
+template <typename T, int NCH, int RW>
 __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long ldx, int8_t* __restrict__ Q, long ldq,
                                                   float* __restrict__ S, long M, int K) {
   const int lane = threadIdx.x & 63;
@@ -60,88 +60,99 @@ __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long 
     if (s > 0.f) return (uint32_t)(int)rintf(fminf(fmaxf(v / s, -127.f), 127.f)) & 255u;
     return 0u;
   };
-  if constexpr (VEC) {
-    const int nch = K >> 3;
-    uint32_t v[RW][NCH > 0 ? NCH : 1][W], top[W];
-    auto load = [&](long row, int ch, uint32_t* o) {
+  const int nch = (K + 7) >> 3;
+  uint32_t v[RW][NCH > 0 ? NCH : 1][W], top[W];
+  auto load = [&](long row, int ch, uint32_t* o) {             // rows of any alignment; zeros past their end
+    const T* at = X + row * ldx + (long)ch * 8;
+    if (ch * 8 + 8 <= K) {
 #pragma unroll
-      for (int p = 0; p < W / 4; ++p)
-        reinterpret_cast<uint4*>(o)[p] = reinterpret_cast<const uint4*>(X + row * ldx + (long)ch * 8)[p];
-    };
-    auto see = [&](const uint32_t* o) {
+      for (int p = 0; p < W / 4; ++p) {
+        const i32x4 w = reinterpret_cast<const any_i32x4*>(at)[p];
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if constexpr (sizeof(T) == 2)
-          top[w] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top[w]), __builtin_bit_cast(u16x2, o[w] & 0x7FFF7FFFu)));
-        else top[w] = max(top[w], o[w] & 0x7FFFFFFFu);
+        for (int e = 0; e < 4; ++e) o[p * 4 + e] = (uint32_t)w[e];
       }
-    };
-    auto store = [&](long row, int ch, const uint32_t* o) {
-      uint32_t w[2];
+    } else {
+      union { T t[8]; uint32_t w[W]; } u;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t c[4];
+      for (int w = 0; w < W; ++w) u.w[w] = 0u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float f;
-          if constexpr (sizeof(T) == 4) f = __uint_as_float(o[h * 4 + e]);
-          else {
-            const f32x2 two = unpack2<T>(o[h * 2 + e / 2]);
-            f = e & 1 ? two.y : two.x;
-          }
-          c[e] = code(f);
+      for (int e = 0; e < 8; ++e)
+        if (ch * 8 + e < K) u.t[e] = at[e];
+#pragma unroll
+      for (int w = 0; w < W; ++w) o[w] = u.w[w];
+    }
+  };
+  auto see = [&](const uint32_t* o) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if constexpr (sizeof(T) == 2)
+        top[w] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top[w]), __builtin_bit_cast(u16x2, o[w] & 0x7FFF7FFFu)));
+      else top[w] = max(top[w], o[w] & 0x7FFFFFFFu);
+    }
+  };
+  auto store = [&](long row, int ch, const uint32_t* o) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f;
+        if constexpr (sizeof(T) == 4) f = __uint_as_float(o[h * 4 + e]);
+        else {
+          const f32x2 two = unpack2<T>(o[h * 2 + e / 2]);
+          f = e & 1 ? two.y : two.x;
         }
-        w[h] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+        c[e] = code(f);
       }
-      *reinterpret_cast<uint2*>(Q + row * ldq + (long)ch * 8) = uint2{w[0], w[1]};
-    };
+      w[h] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+    }
+    int8_t* at = Q + row * ldq + (long)ch * 8;
+    typedef uint32_t two __attribute__((ext_vector_type(2)));
+    typedef two any_two __attribute__((aligned(1)));
+    if (ch * 8 + 8 <= K) *reinterpret_cast<any_two*>(at) = two{w[0], w[1]};
+    else
+      for (int e = 0; ch * 8 + e < K; ++e) at[e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
+  };
+  if constexpr (NCH > 0) {
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (lane + 64 * i < nch) load(min(row0 + r, M - 1), lane + 64 * i, v[r][i]);
+  }
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const long row = row0 + r;
+    if (row >= M) return;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top[w] = 0u;
     if constexpr (NCH > 0) {
 #pragma unroll
-      for (int r = 0; r < RW; ++r)
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (lane + 64 * i < nch) load(min(row0 + r, M - 1), lane + 64 * i, v[r][i]);
-    }
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      const long row = row0 + r;
-      if (row >= M) return;
-#pragma unroll
-      for (int w = 0; w < W; ++w) top[w] = 0u;
-      if constexpr (NCH > 0) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (lane + 64 * i < nch) see(v[r][i]);
-      } else {
-        for (int ch = lane; ch < nch; ch += 64) {
-          load(row, ch, v[0][0]);
-          see(v[0][0]);
-        }
-      }
-      uint32_t m = 0u;
-#pragma unroll
-      for (int w = 0; w < W; ++w) m = max(m, sizeof(T) == 2 ? max(top[w] & 0xFFFFu, top[w] >> 16) : top[w]);
-      m = wave_umax(m);
-      if constexpr (sizeof(T) == 4) scale(row, __uint_as_float(m));
-      else scale(row, unpack2<T>(m).x);
-      if constexpr (NCH > 0) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (lane + 64 * i < nch) store(row, lane + 64 * i, v[r][i]);
-      } else {
-        for (int ch = lane; ch < nch; ch += 64) {
-          load(row, ch, v[0][0]);
-          store(row, ch, v[0][0]);
-        }
+      for (int i = 0; i < NCH; ++i)
+        if (lane + 64 * i < nch) see(v[r][i]);
+    } else {
+      for (int ch = lane; ch < nch; ch += 64) {
+        load(row, ch, v[0][0]);
+        see(v[0][0]);
       }
     }
-  } else {
-    static_assert(RW == 1, "rows of any alignment: one a wave");
-    const T* x = X + row0 * ldx;
     uint32_t m = 0u;
-    for (int k = lane; k < K; k += 64) m = max(m, __float_as_uint(to_f(x[k])) & 0x7FFFFFFFu);
-    scale(row0, __uint_as_float(wave_umax(m)));
-    for (int k = lane; k < K; k += 64) Q[row0 * ldq + k] = (int8_t)code(to_f(x[k]));
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = max(m, sizeof(T) == 2 ? max(top[w] & 0xFFFFu, top[w] >> 16) : top[w]);
+    m = wave_umax(m);
+    if constexpr (sizeof(T) == 4) scale(row, __uint_as_float(m));
+    else scale(row, unpack2<T>(m).x);
+    if constexpr (NCH > 0) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (lane + 64 * i < nch) store(row, lane + 64 * i, v[r][i]);
+    } else {
+      for (int ch = lane; ch < nch; ch += 64) {
+        load(row, ch, v[0][0]);
+        store(row, ch, v[0][0]);
+      }
+    }
   }
 }
 
@@ -240,7 +251,11 @@ struct ScaleEpi {
   }
 };
 
+// rows that the tiled kernel can read as they are: aligned, and of whole chunks.  Tokens may end inside a chunk where the
+// weights (or their copy) hold zeros there: whatever lies behind the codes is a finite integer and is multiplied by zero.
+// (An aligned chunk that holds a code lies in that code's page.)
 static bool rows_ok(const void* p, long ld, long K) { return al16(p) && ld % 16 == 0 && K % 16 == 0; }
+static bool tokens_ok(const void* p, long ld, long K) { return al16(p) && ld % 16 == 0 && ld >= up16(K); }
 static bool bad_dims(long M, long N, long K) {
   return M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00L || N > 0x7fffff00L || K > 131071;
 }
@@ -258,24 +273,22 @@ extern "C" int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long 
   SVK_DISPATCH_DTYPE(dtype, T, {
     const T* x = (const T*)X;
     int8_t* q = (int8_t*)Q;
-    auto go = [&](auto nch, auto rw, auto vec) {
+    auto go = [&](auto nch, auto rw) {
       constexpr int RW = decltype(rw)::value;
-      hipLaunchKernelGGL((quant_rows<T, decltype(nch)::value, RW, decltype(vec)::value>), dim3((unsigned)((M + 4 * RW - 1) / (4 * RW))),
+      hipLaunchKernelGGL((quant_rows<T, decltype(nch)::value, RW>), dim3((unsigned)((M + 4 * RW - 1) / (4 * RW))),
                          dim3(256), 0, st, x, ldx, q, ldq, S, M, (int)K);
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
-    const bool vec = K % 8 == 0 && al16(X) && ldx * (long)sizeof(T) % 16 == 0 && ((uintptr_t)Q & 7) == 0 && ldq % 8 == 0;
     // short rows in numbers: several a wave, whose loads are under way together
     const bool many = M >= 4096;
-    if (!vec) go(I0{}, I1{}, std::false_type{});
-    else if (K <= 512) many ? go(I1{}, I4{}, std::true_type{}) : go(I1{}, I1{}, std::true_type{});
-    else if (K <= 1024) many ? go(I2{}, I2{}, std::true_type{}) : go(I2{}, I1{}, std::true_type{});
-    else if (K <= 2048) go(I4{}, I1{}, std::true_type{});
-    else if (K <= 4096) go(std::integral_constant<int, 8>{}, I1{}, std::true_type{});
-    else go(I0{}, I1{}, std::true_type{});
+    if (K <= 512) many ? go(I1{}, I4{}) : go(I1{}, I1{});
+    else if (K <= 1024) many ? go(I2{}, I2{}) : go(I2{}, I1{});
+    else if (K <= 2048) go(I4{}, I1{});
+    else if (K <= 4096) go(std::integral_constant<int, 8>{}, I1{});
+    else go(I0{}, I1{});
     return check_launch("quant_rows");
   });
 }
@@ -283,7 +296,7 @@ extern "C" int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long 
 extern "C" long svk_gemm_i8_workspace(const void* A, long lda, const void* W, long ldw, long M, long N, long K) {
   if (bad_dims(M, N, K) || M <= SKINNY_M) return 0;
   const long ldk = up16(K);
-  return (rows_ok(A, lda, K) ? 0 : M * ldk) + (rows_ok(W, ldw, K) ? 0 : N * ldk);
+  return (tokens_ok(A, lda, K) ? 0 : M * ldk) + (rows_ok(W, ldw, K) ? 0 : N * ldk);
 }
 
 extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, const void* W, long ldw, const float* sw,
@@ -306,28 +319,21 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
     const bool past = al16(Y) && ldy * (long)sizeof(T) % 16 == 0 && N * (long)sizeof(T) % 16 == 0;
     Args p{(const char*)A, (const char*)W, lda, ldw, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
-      const bool vec = rows_ok(A, lda, K) && rows_ok(W, ldw, K);
       ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0, past};
-      return few_tokens<int8_t, 1>(p, vec, N, epi, st, "gemm_i8_few");
+      return few_tokens<int8_t, 1>(p, N, epi, st, "gemm_i8_few");
     }
     char* at = (char*)ws;
-    auto pad = [&](const void* X, long ld, long rows) {
-      const unsigned blocks = (unsigned)std::min<long>((rows * ldk + 255) / 256, 8192);
-      hipLaunchKernelGGL((pad_rows<int8_t>), dim3(blocks), dim3(256), 0, st, (const int8_t*)X, ld, (int8_t*)at, ldk, rows, (int)K);
-      return check_launch("pad_rows");
-    };
-    if (!rows_ok(A, lda, K)) {
-      if (int rc = pad(A, lda, M)) return rc;
+    if (!tokens_ok(A, lda, K)) {
+      if (int rc = pad<int8_t>(A, lda, at, M, K, st)) return rc;
       p.A = at;
       p.lda = ldk;
       at += M * ldk;
-      p.K = (int)ldk;
     }
+    p.K = (int)ldk;                                 // whole chunks
     if (!rows_ok(W, ldw, K)) {
-      if (int rc = pad(W, ldw, N)) return rc;
+      if (int rc = pad<int8_t>(W, ldw, at, N, K, st)) return rc;
       p.B = at;
       p.ldb = ldk;
-      p.K = (int)ldk;
     }
     p.nk = stages<int8_t>(p.K);
     p.abytes = (M - 1) * p.lda + p.K;

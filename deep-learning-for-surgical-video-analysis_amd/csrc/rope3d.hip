@@ -9,7 +9,7 @@
 // The angle is formed in 64 bits and reduced to a fraction of a turn there (a frame number of 1e5 times f = 1 has no
 // useful fraction left in f32), the sine and cosine of the reduced angle in f32.  A workgroup forms the R pairs of its
 // tokens once, in LDS, for all heads of q and k: 2 R sines a token against (Hq + Hk) hd values moved.
-// Bound by HBM: q and k are read once and written once, as 16-byte pieces where rows allow it.
+// Bound by HBM: q and k are read once and written once, as 16-byte pieces.
 #include "svk_common.h"
 #include <algorithm>
 
@@ -28,14 +28,46 @@ struct RopeArgs {
   long ldp, sbp;                // values between tokens / batches (sbp 0: one table for all)
   const double* freqs;
   int nt, nh, R, hd, N, tokens, tpb;
+  bool apart;                   // the outputs are not the inputs
   float sign;
 };
 
-// V channels a unit (a pair of V-channel pieces in the halves layout's rotated part)
-template <typename T, typename P, int V, bool IL>
-__global__ __launch_bounds__(256) void rope3d(RopeArgs a) {
-  extern __shared__ float2 cs[];                                // [tokens of the workgroup][R]: cos, sin
+// n values (V where n >= V) of any alignment
+template <typename T, int V>
+__device__ __forceinline__ void get(const T* p, int n, float* v) {
   typedef T vec __attribute__((ext_vector_type(V)));
+  typedef vec anywhere __attribute__((aligned(sizeof(T))));
+  if (n >= V) {
+    const vec w = *reinterpret_cast<const anywhere*>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = to_f(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < n ? to_f(p[e]) : 0.f;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void set(T* p, int n, const float* v) {
+  typedef T vec __attribute__((ext_vector_type(V)));
+  typedef vec anywhere __attribute__((aligned(sizeof(T))));
+  if (n >= V) {
+    vec w;
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = from_f<T>(v[e]);
+    *reinterpret_cast<anywhere*>(p) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < n) p[e] = from_f<T>(v[e]);
+  }
+}
+
+// A unit: V channels, 16 bytes (V pairs of the halves layout: two pieces), fewer at the end of a part of the head (WHOLE:
+// nowhere).  Pieces need no alignment (pairs 19 apart in heads of 72, 161 MB: 41 us, value by value 142).
+template <typename T, typename P, bool IL, bool WHOLE>
+__global__ __launch_bounds__(256) void rope3d(RopeArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  extern __shared__ float2 cs[];                                // [tokens of the workgroup][R]: cos, sin
   const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.tokens - t0);
   for (int i = threadIdx.x; i < nt * a.R; i += 256) {
     const int t = i / a.R, r = i - t * a.R, tok = t0 + t, b = tok / a.N, n = tok - b * a.N;
@@ -48,8 +80,8 @@ __global__ __launch_bounds__(256) void rope3d(RopeArgs a) {
     cs[i] = float2{c, a.sign * s};
   }
   __syncthreads();
-  const int rot = IL ? 2 * a.R / V : a.R / V;                   // units of a head's rotated part
-  const int uph = rot + (a.hd - 2 * a.R) / V, upt = uph * (a.q.heads + a.k.heads);
+  const int part = IL ? 2 * a.R : a.R, rot = (part + V - 1) / V;       // units of a head's rotated part
+  const int uph = rot + (a.hd - 2 * a.R + V - 1) / V, upt = uph * (a.q.heads + a.k.heads);
   for (int u = threadIdx.x; u < nt * upt; u += 256) {
     const int t = u / upt, v = u - t * upt;
     int h = v / uph;
@@ -60,47 +92,57 @@ __global__ __launch_bounds__(256) void rope3d(RopeArgs a) {
     const T* x = reinterpret_cast<const T*>(m.x) + b * m.sbx + n * m.ldx + (long)h * a.hd;
     T* y = reinterpret_cast<T*>(m.y) + b * m.sby + n * m.ldy + (long)h * a.hd;
     const float2* z = cs + t * a.R;
-    if (w >= rot) {
-      const int c = 2 * a.R + (w - rot) * V;
-      *reinterpret_cast<vec*>(y + c) = *reinterpret_cast<const vec*>(x + c);
-    } else if constexpr (IL) {
-      const int c = w * V;
-      const vec p = *reinterpret_cast<const vec*>(x + c);
-      vec o;
+    float p[V], q[V], o[V];
+    if (w >= rot) {                                             // past the pairs: the values themselves
+      if (x == y) continue;                                     // in place: there already
+      int c = 2 * a.R + (w - rot) * V;
+      if (!WHOLE && c + V > a.hd && a.hd - V >= 2 * a.R) c = a.hd - V;       // the last piece: a whole one that overlaps
+      const int left = a.hd - c;
+      typedef uint32_t four __attribute__((ext_vector_type(4)));
+      typedef four anywhere __attribute__((aligned(2)));
+      if (WHOLE || left >= V) *reinterpret_cast<anywhere*>(y + c) = *reinterpret_cast<const anywhere*>(x + c);
+      else
+        for (int e = 0; e < left; ++e) y[c + e] = x[c + e];
+      continue;
+    }
+    int c = w * V;
+    // the last piece of the rotated part: a whole one that overlaps the one before, unless that is being turned in place
+    if (!WHOLE && a.apart && c + V > part && part >= V) c = part - V;
+    if constexpr (IL) {
+      get<T, V>(x + c, WHOLE ? V : part - c, p);
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const float2 r = z[(c + e) >> 1];
-        const float f = to_f(p[e]), g = to_f(p[e + 1]);
-        o[e] = from_f<T>(f * r.x - g * r.y);
-        o[e + 1] = from_f<T>(f * r.y + g * r.x);
+        const float2 r = z[WHOLE ? (c + e) >> 1 : min((c + e) >> 1, a.R - 1)];
+        o[e] = p[e] * r.x - p[e + 1] * r.y;
+        o[e + 1] = p[e] * r.y + p[e + 1] * r.x;
       }
-      *reinterpret_cast<vec*>(y + c) = o;
+      set<T, V>(y + c, WHOLE ? V : part - c, o);
     } else {
-      const int c = w * V;
-      const vec p = *reinterpret_cast<const vec*>(x + c), q = *reinterpret_cast<const vec*>(x + a.R + c);
-      vec o, s;
+      get<T, V>(x + c, WHOLE ? V : part - c, p);
+      get<T, V>(x + a.R + c, WHOLE ? V : part - c, q);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float2 r = z[c + e];
-        const float f = to_f(p[e]), g = to_f(q[e]);
-        o[e] = from_f<T>(f * r.x - g * r.y);
-        s[e] = from_f<T>(f * r.y + g * r.x);
+        const float2 r = z[WHOLE ? c + e : min(c + e, a.R - 1)];
+        const float f = p[e], g = q[e];
+        o[e] = f * r.x - g * r.y;
+        q[e] = f * r.y + g * r.x;
       }
-      *reinterpret_cast<vec*>(y + c) = o;
-      *reinterpret_cast<vec*>(y + a.R + c) = s;
+      set<T, V>(y + c, WHOLE ? V : part - c, o);
+      set<T, V>(y + a.R + c, WHOLE ? V : part - c, q);
     }
   }
 }
 
 template <typename T, typename P>
-static int launch(const RopeArgs& a, bool vec, bool il, hipStream_t st) {
+static int launch(const RopeArgs& a, bool il, hipStream_t st) {
   const dim3 grid((unsigned)((a.tokens + a.tpb - 1) / a.tpb)), block(256);
   const size_t lds = (size_t)a.tpb * a.R * sizeof(float2);
   constexpr int V = 16 / (int)sizeof(T);
-  if (vec && il) hipLaunchKernelGGL((rope3d<T, P, V, true>), grid, block, lds, st, a);
-  else if (vec) hipLaunchKernelGGL((rope3d<T, P, V, false>), grid, block, lds, st, a);
-  else if (il) hipLaunchKernelGGL((rope3d<T, P, 2, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((rope3d<T, P, 1, false>), grid, block, lds, st, a);
+  const bool whole = (il ? 2 * a.R : a.R) % V == 0 && (a.hd - 2 * a.R) % V == 0;
+  if (il && whole) hipLaunchKernelGGL((rope3d<T, P, true, true>), grid, block, lds, st, a);
+  else if (il) hipLaunchKernelGGL((rope3d<T, P, true, false>), grid, block, lds, st, a);
+  else if (whole) hipLaunchKernelGGL((rope3d<T, P, false, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((rope3d<T, P, false, false>), grid, block, lds, st, a);
   return check_launch("rope3d");
 }
 
@@ -132,26 +174,15 @@ extern "C" int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo
     a.pos = (const char*)pos;
     a.ldp = ldp; a.sbp = sbp; a.freqs = freqs;
     a.nt = nt; a.nh = nh; a.R = R; a.hd = hd; a.N = N; a.tokens = B * N;
+    a.apart = Qo != Q && (!kv_heads || Ko != K);
     a.sign = inverse ? -1.f : 1.f;
     constexpr int V = 16 / (int)sizeof(T);
-    auto ok = [&](const Map& m) {
-      return !m.heads || (((((uintptr_t)m.x) | ((uintptr_t)m.y)) & 15) == 0 && (m.ldx | m.sbx | m.ldy | m.sby) % V == 0);
-    };
-    const bool vec = hd % V == 0 && (interleaved ? 2 * R : R) % V == 0 && (hd - 2 * R) % V == 0 && ok(a.q) && ok(a.k);
-    // interleaved pairs are moved two values at a time where 16-byte pieces do not fit; that needs even rows
-    auto even = [&](const Map& m) {
-      return !m.heads || (((((uintptr_t)m.x) | ((uintptr_t)m.y)) & (2 * sizeof(T) - 1)) == 0 && (m.ldx | m.sbx | m.ldy | m.sby) % 2 == 0);
-    };
-    if (interleaved && !vec && !(hd % 2 == 0 && even(a.q) && even(a.k))) {
-      set_error("svk_rope3d: interleaved pairs need an even head width, even strides and pair-aligned pointers");
-      return SVK_EUNSUPPORTED;
-    }
     // about 1024 units (4 a thread) a workgroup, fewer where that would leave CUs idle; the table within 32 KiB of LDS
-    const long upt = (long)(heads + kv_heads) * (vec ? hd / V : hd);
+    const long upt = (long)(heads + kv_heads) * ((hd + V - 1) / V);
     long tpb = std::min<long>(std::max<long>(1, 1024 / upt), std::max<long>(1, a.tokens / 2048));
     a.tpb = (int)std::max<long>(1, std::min<long>(tpb, 4096 / R));
-    if (pos_type == SVK_POS_I32) return launch<T, int>(a, vec, interleaved, (hipStream_t)stream);
-    if (pos_type == SVK_POS_I64) return launch<T, long>(a, vec, interleaved, (hipStream_t)stream);
-    return launch<T, float>(a, vec, interleaved, (hipStream_t)stream);
+    if (pos_type == SVK_POS_I32) return launch<T, int>(a, interleaved, (hipStream_t)stream);
+    if (pos_type == SVK_POS_I64) return launch<T, long>(a, interleaved, (hipStream_t)stream);
+    return launch<T, float>(a, interleaved, (hipStream_t)stream);
   });
 }

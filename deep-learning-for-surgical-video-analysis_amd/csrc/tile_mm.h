@@ -442,30 +442,30 @@ template <typename T> inline int stages(long k) { return (int)((k * (long)sizeof
 
 // Few token rows against the weights: each weight value is read once, straight into registers, and the reduction is
 // split over the workgroup's waves and joined in LDS.  MT blocks of 16 tokens, NB blocks of 16 weight rows a workgroup
-// (the epilogue's map names them, `epi.per` results).  VEC: rows 16-byte aligned and whole 16-byte chunks; otherwise
-// chunks are put together value by value.  Bound by the weights' bytes, and below some MiB by one trip to memory.
+// (the epilogue's map names them, `epi.per` results).  Rows of any alignment and length.  Bound by the weights' bytes, and below some MiB by one trip to memory.
 constexpr int SK_WAVES = 8;
 constexpr int SKINNY_M = 64;
 
-template <typename T, bool VEC>
+// 16 bytes of a row from byte kb on, zeros past its end; rows of any alignment (the hardware reads 16 bytes anywhere)
+typedef i32x4 any_i32x4 __attribute__((aligned(1)));
+template <typename T>
 __device__ __forceinline__ i32x4 load_chunk(const char* row, long kb, long kbytes) {
   constexpr int ES = sizeof(T);
-  if constexpr (VEC) {
-    return kb < kbytes ? *reinterpret_cast<const i32x4*>(row + kb) : i32x4{0, 0, 0, 0};
-  } else {
-    union { i32x4 v; T e[16 / ES]; } u;
-    u.v = i32x4{0, 0, 0, 0};
+  if (kb + 16 <= kbytes) return *reinterpret_cast<const any_i32x4*>(row + kb);
+  union { i32x4 v; T e[16 / ES]; } u;
+  u.v = i32x4{0, 0, 0, 0};
+  if (kb < kbytes)
 #pragma unroll
     for (int i = 0; i < 16 / ES; ++i)
       if (kb + i * ES < kbytes) u.e[i] = *reinterpret_cast<const T*>(row + kb + i * ES);
-    return u.v;
-  }
+  return u.v;
 }
 
-template <typename T, int MT, int NB, bool VEC, class Epi>
+// ENDS: rows that end inside a 16-byte chunk
+template <typename T, int MT, int NB, bool ENDS, class Epi>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_mm(Args p, Epi epi) {
   typedef typename Acc<T>::t acc_t;
-  constexpr int U = !VEC ? 1 : (MT + NB <= 2 ? 8 : (MT + NB <= 5 ? 4 : 2));        // 64-byte steps in flight
+  constexpr int U = MT + NB <= 2 ? 8 : (MT + NB <= 5 ? 4 : 2);  // 64-byte steps in flight
   typedef std::conditional_t<std::is_same<T, int8_t>::value, int, float> sum_t;
   __shared__ sum_t red[SK_WAVES][MT][NB][16][17];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -484,14 +484,22 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_mm(Args p, Epi epi) {
     for (int j = 0; j < NB; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
   for (long kb = (long)wave * 64 * U; kb < kbytes; kb += (long)SK_WAVES * 64 * U) {
     i32x4 fb[U][NB], fa[U][MT];
+    auto load = [&](auto E) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long k = kb + u * 64 + fq * 16;
+      for (int u = 0; u < U; ++u) {
+        const long k = kb + u * 64 + fq * 16;
+        auto get = [&](const char* row) {
+          if constexpr (decltype(E)::value) return load_chunk<T>(row, k, kbytes);
+          else return k < kbytes ? *reinterpret_cast<const any_i32x4*>(row + k) : i32x4{0, 0, 0, 0};
+        };
 #pragma unroll
-      for (int j = 0; j < NB; ++j) fb[u][j] = load_chunk<T, VEC>(rb[j], k, kbytes);
+        for (int j = 0; j < NB; ++j) fb[u][j] = get(rb[j]);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) fa[u][i] = load_chunk<T, VEC>(ra[i], k, kbytes);
-    }
+        for (int i = 0; i < MT; ++i) fa[u][i] = get(ra[i]);
+      }
+    };
+    if (ENDS && kb + U * 64 > kbytes) load(std::true_type{});      // the turn in which the rows end
+    else load(std::false_type{});
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -523,14 +531,14 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_mm(Args p, Epi epi) {
 // (2 x 5632 rows of 2048 in bf16, 16 tokens: 32 rows a workgroup 15.5, 16 rows 14, 44 rows 11.3 us: 46 MB of weights at
 // 4.1 TB/s)
 template <typename T, int MT, int WPR, class Epi>
-static int launch_skinny(const Args& p, bool vec, long results, Epi epi, hipStream_t st, const char* name) {
+static int launch_skinny(const Args& p, long results, Epi epi, hipStream_t st, const char* name) {
   long per = (results + 255) / 256;
   per = per < 16 / WPR ? 16 / WPR : (per > 64 / WPR ? 64 / WPR : per);
   epi.per = (int)per;
   const dim3 grid((unsigned)((results + per - 1) / per)), block(64 * SK_WAVES);
   auto go = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
-    if (vec) hipLaunchKernelGGL((skinny_mm<T, MT, NB, true, Epi>), grid, block, 0, st, p, epi);
+    if (p.K * sizeof(T) % 16) hipLaunchKernelGGL((skinny_mm<T, MT, NB, true, Epi>), grid, block, 0, st, p, epi);
     else hipLaunchKernelGGL((skinny_mm<T, MT, NB, false, Epi>), grid, block, 0, st, p, epi);
     set_last_kernel(name);
     return check_launch(name);
@@ -543,22 +551,29 @@ static int launch_skinny(const Args& p, bool vec, long results, Epi epi, hipStre
   }
 }
 template <typename T, int WPR, class Epi>
-static int few_tokens(const Args& p, bool vec, long results, const Epi& epi, hipStream_t st, const char* name) {
-  if (p.M <= 16) return launch_skinny<T, 1, WPR>(p, vec, results, epi, st, name);
-  if (p.M <= 32) return launch_skinny<T, 2, WPR>(p, vec, results, epi, st, name);
-  return launch_skinny<T, 4, WPR>(p, vec, results, epi, st, name);
+static int few_tokens(const Args& p, long results, const Epi& epi, hipStream_t st, const char* name) {
+  if (p.M <= 16) return launch_skinny<T, 1, WPR>(p, results, epi, st, name);
+  if (p.M <= 32) return launch_skinny<T, 2, WPR>(p, results, epi, st, name);
+  return launch_skinny<T, 4, WPR>(p, results, epi, st, name);
 }
 
-// copy of rows of `width` values into rows of `ld` values (a multiple of 16 bytes), the rest filled with zeros: what
-// the tiled kernels read where a row operand's length or address is no whole number of 16-byte chunks
+// copy of rows into rows of whole 16-byte chunks, the last filled up with zeros: what the tiled kernels read where a row
+// operand's length or address is no whole number of chunks.  A chunk a thread, rows read at any alignment (value by value
+// it took longer than the product: 315 x 3930 x 4240 in 8 bits 72 us in all, by chunks 63; 38 with the tokens quantised 8 values a lane too)
 template <typename T>
-__global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ X, long ldx, T* __restrict__ Y, long ld, long rows,
-                                                int width) {
-  const long total = rows * ld;
+__global__ __launch_bounds__(256) void pad_rows(const char* __restrict__ X, long ldx, char* __restrict__ Y, long rows, long kbytes) {
+  const long chunks = (kbytes + 15) / 16, total = rows * chunks;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    const long r = i / ld, c = i - r * ld;
-    Y[i] = c < width ? X[r * ldx + c] : T(0);
+    const long r = total <= 0x7fffffffL ? (uint32_t)i / (uint32_t)chunks : i / chunks, c = i - r * chunks;
+    *reinterpret_cast<i32x4*>(Y + i * 16) = load_chunk<T>(X + r * ldx, c * 16, kbytes);
   }
+}
+// ldx: bytes between the rows of X
+template <typename T>
+static int pad(const void* X, long ldx, void* Y, long rows, long kbytes, hipStream_t st) {
+  const long blocks = (rows * ((kbytes + 15) / 16) + 255) / 256;
+  hipLaunchKernelGGL((pad_rows<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, (const char*)X, ldx, (char*)Y, rows, kbytes);
+  return check_launch("pad_rows");
 }
 
 inline long up16(long bytes) { return (bytes + 15) & ~15L; }

@@ -67,7 +67,8 @@ def _rope_close(got, x, pos, freqs, sections, heads, il, inverse):
 @pytest.mark.parametrize("il", [False, True])
 @pytest.mark.parametrize("B,N,heads,kv,hd,sections", [
     (1, 1, 1, 1, 6, (1, 1, 1)), (2, 49, 8, 8, 64, (8, 12, 12)), (3, 17, 6, 2, 80, (10, 10, 10)),
-    (2, 130, 3, 3, 40, (4, 8, 8)), (1, 2049, 2, 1, 34, (0, 5, 6)), (5, 3, 1, 1, 128, (64, 0, 0)), (1, 7, 2, 2, 18, (3, 3, 3))])
+    (2, 130, 3, 3, 40, (4, 8, 8)), (1, 2049, 2, 1, 34, (0, 5, 6)), (5, 3, 1, 1, 128, (64, 0, 0)), (1, 7, 2, 2, 18, (3, 3, 3)),
+    (2, 40, 4, 4, 72, (7, 6, 6)), (1, 11, 3, 1, 9, (2, 1, 1)), (2, 5, 1, 1, 33, (5, 5, 6)), (1, 300, 5, 5, 7, (1, 1, 1))])
 def test_rope3d(cuda, dt, il, B, N, heads, kv, hd, sections):
     ops = _ops()
     q, k = _rand(B, N, heads * hd, dt=dt, seed=1), _rand(B, N, kv * hd, dt=dt, seed=2)
@@ -166,9 +167,6 @@ def test_rope3d_refusals(cuda):
     for kw in bad:
         with pytest.raises(svk.SvkError):
             ok(**kw)
-    odd = torch.zeros(1, 2, 9, device="cuda")
-    with pytest.raises(svk.SvkError, match="interleaved"):
-        ops.rope3d(odd, None, pos[:2], f[:4].contiguous(), (2, 1, 1), 1, interleaved=True)
 
 
 # ---------------------------------------------------------------- gated feed-forward
@@ -501,6 +499,23 @@ def test_gemm_i8_exact_sums_views_and_extremes(cuda):
         assert bool(y[1].isnan().all()) and bool(y[0].isfinite().all())
     e = ops.gemm_i8(_codes(4, 16, 1)[:0], one(0), _codes(5, 16, 2), one(5))
     assert e.shape == (0, 5) and e.dtype == torch.float16
+
+
+@pytest.mark.parametrize("K", [61, 333, 1001])
+def test_gemm_i8_tokens_that_end_inside_a_chunk(cuda, K):
+    """Codes of quant_rows keep whatever their buffer held behind a row of K % 16 values; it must not be seen."""
+    ops = _ops()
+    M, N = 100, 72
+    buf = torch.full((M, (K + 15) // 16 * 16), 77, dtype=torch.int8, device="cuda")
+    a, w = buf[:, :K], _codes(N, K, 2)
+    a.copy_(_codes(M, K, 1))
+    one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+    want = a.to(F64) @ w.to(F64).t()
+    assert torch.equal(ops.gemm_i8(a, one(M), w, one(N), dtype=torch.float32).to(F64), want)
+    wb = torch.full((N, (K + 15) // 16 * 16), -55, dtype=torch.int8, device="cuda")
+    wb[:, :K] = w
+    assert torch.equal(ops.gemm_i8(a, one(M), wb[:, :K], one(N), dtype=torch.float32).to(F64), want)
+    assert torch.equal(ops.gemm_i8(a[:5], one(5), wb[:, :K], one(N), dtype=torch.float32).to(F64), want[:5])
 
 
 def test_i8_refusals(cuda):
