@@ -172,9 +172,10 @@ struct ScaleEpi {
 
   __device__ __forceinline__ float value(int acc, float a, float w, float b) const {
     const float v = (float)acc * a * w + b;
-    if constexpr (sizeof(T) == 4) return apply_act(v, ACT < 0 ? act : ACT);
-    else if constexpr (ACT == SVK_ACT_GELU) return gelu16(v);
-    else return apply_act_fast(v, ACT < 0 ? act : ACT);
+    const int f = ACT < 0 ? act : ACT;
+    if (f == SVK_ACT_RELU) return v < 0.f ? 0.f : v;            // NaN stays NaN
+    if constexpr (sizeof(T) == 4) return apply_act(v, f);
+    else return f == SVK_ACT_GELU ? gelu16(v) : apply_act_fast(v, f);
   }
   template <class C> __device__ __forceinline__ long first(int tn) const { return (long)tn * C::BN; }
   template <class C> __device__ __forceinline__ uint32_t offset(int r, uint32_t ldb) const { return (uint32_t)pair_col(r) * ldb; }

@@ -501,6 +501,19 @@ def test_gemm_i8_exact_sums_views_and_extremes(cuda):
     assert e.shape == (0, 5) and e.dtype == torch.float16
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "tanh"])
+@pytest.mark.parametrize("M", [5, 100])
+def test_gemm_i8_not_finite_tokens_are_nan_behind_every_activation(cuda, dt, act, M):
+    ops = _ops()
+    x, w = _rand(M, 64, dt=torch.float32, seed=1), ops.quant_rows(_rand(48, 64, dt=torch.float32, seed=2))
+    clean = ops.gemm_i8(*ops.quant_rows(x), *w, act=act, dtype=dt)
+    x[2, 7], x[4, 0] = float("inf"), float("nan")
+    got = ops.gemm_i8(*ops.quant_rows(x), *w, act=act, dtype=dt)
+    rest = [i for i in range(M) if i not in (2, 4)]
+    assert torch.equal(got[rest], clean[rest]) and bool(got[[2, 4]].isnan().all())
+
+
 @pytest.mark.parametrize("K", [61, 333, 1001])
 def test_gemm_i8_tokens_that_end_inside_a_chunk(cuda, K):
     """Codes of quant_rows keep whatever their buffer held behind a row of K % 16 values; it must not be seen."""
