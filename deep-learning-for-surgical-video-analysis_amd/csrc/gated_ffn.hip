@@ -350,7 +350,8 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     set_error("svk_gated_ffn: weights or 256 rows of x of 4 GiB or more");
     return SVK_EUNSUPPORTED;
   }
-  if (ws_bytes < svk_gated_ffn_workspace(dtype, X, ldx, W, ldw, M, H, K)) { set_error("svk_gated_ffn: workspace too small"); return SVK_EINVAL; }
+  const long need = svk_gated_ffn_workspace(dtype, X, ldx, W, ldw, M, H, K);
+  if (need && (!ws || !al16(ws) || ws_bytes < need)) { set_error("svk_gated_ffn: workspace too small or misaligned"); return SVK_EINVAL; }
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {

@@ -313,7 +313,8 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
     set_error("svk_gemm_i8: weights or 256 rows of a of 4 GiB or more");
     return SVK_EUNSUPPORTED;
   }
-  if (ws_bytes < svk_gemm_i8_workspace(A, lda, W, ldw, M, N, K)) { set_error("svk_gemm_i8: workspace too small"); return SVK_EINVAL; }
+  const long need = svk_gemm_i8_workspace(A, lda, W, ldw, M, N, K);
+  if (need && (!ws || !al16(ws) || ws_bytes < need)) { set_error("svk_gemm_i8: workspace too small or misaligned"); return SVK_EINVAL; }
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {

@@ -66,6 +66,14 @@ def test_gated_ffn_sizes():
         assert (lib.svk_gemm_i8_workspace(A, 63, A, 63, M, 64, 63) == 0) == (want == 0)
 
 
+@pytest.mark.parametrize("ws,n", [(None, 1 << 30), (A + 8, 1 << 30), (A, (100 + 64) * 128 - 1)])
+def test_workspaces_that_are_missing_misaligned_or_short(ws, n):
+    lib = _lib()
+    odd = dict(K=63, ldx=63, ldw=63)                                 # 100 + 64 rows padded to 128 bytes
+    assert _gated(lib, ws=ws, n=n, **odd) == -1 and b"workspace" in lib.svk_last_error()
+    assert _i8(lib, K=127, lda=127, ldw=127, N=64, ldy=64, ws=ws, n=n) == -1 and b"workspace" in lib.svk_last_error()
+
+
 def _gated_bwd(lib, **kw):
     a = dict(dt=0, x=A, w=A, pre=A, dh=A, lddh=32, dx=A, lddx=64, dw=A, db=A, M=100, H=32, K=64, act=0, ws=A, n=1 << 30)
     a.update(kw)
