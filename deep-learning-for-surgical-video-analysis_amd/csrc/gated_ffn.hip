@@ -306,8 +306,8 @@ struct BwdWs {
     w = padx ? up16(2 * H * ldk) : 0;
     rows = dpre_rows(M, H);
     sums = db ? up16((M + rows - 1) / rows * 2 * H * 4) : 0;
-    if (dx) px = plan(M, K, 2 * H);
-    if (dw) pw = plan(2 * H, K, M);
+    if (dx && M) px = plan(M, K, 2 * H);
+    if (dw && M) pw = plan(2 * H, K, M);      // (no tokens: nothing to plan)
     xslabs = px.parts > 1 ? up16(px.parts * M * K * 4) : 0;
     wslabs = pw.parts > 1 ? up16(pw.parts * 2 * H * K * 4) : 0;
     total = dpre + x + w + sums + xslabs + wslabs;

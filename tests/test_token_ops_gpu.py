@@ -341,6 +341,19 @@ def test_gated_ffn_no_tokens(cuda, dt):
     assert dx.shape == (0, 16) and not bool(dw.any()) and not bool(db.any()) and dw.dtype == dt
 
 
+def test_gated_ffn_bwd_entry_without_tokens(cuda):
+    """The C entry itself: sums over no tokens are zeros, written to dW and db."""
+    from svk import _lib
+    lib = _lib.load()
+    x, w = torch.zeros(1, 16, device="cuda"), torch.zeros(24, 16, device="cuda")
+    dw, db = torch.ones(24, 16, device="cuda"), torch.ones(24, device="cuda")
+    p = x.data_ptr()
+    rc = lib.svk_gated_ffn_bwd(0, p, 16, w.data_ptr(), 16, p, p, 12, p, 16, dw.data_ptr(), db.data_ptr(), 0, 12, 16, 0, None,
+                               0, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0 and not bool(dw.any()) and not bool(db.any())
+
+
 @pytest.mark.parametrize("M", [5, 100])
 def test_gated_ffn_not_finite_stays_in_its_row(cuda, M):
     """A token that holds an infinity or a NaN spoils its own row only (also the rows that share its tile)."""
