@@ -33,19 +33,22 @@ __device__ __forceinline__ float glu_act(float g, int act) {
   }
   return g > 0.f ? g : (g <= 0.f ? 0.f : g);     // NaN stays NaN
 }
-// act(g) and act'(g)
+// act(g) and act'(g) of a kept projection.  Where it left f16's range it is an infinity: act(-inf) is 0, act' there 0 or 1
+// (from 1e4 on act' is 0 or 1 in f32 as well); NaN stays NaN
 template <typename T>
 __device__ __forceinline__ void glu_grad(float g, int act, float& a, float& d) {
+  g = g < -1e4f && act != SVK_GLU_RELU ? -1e4f : g;
+  const float b = g > 1e4f ? 1e4f : g;
   if (act == SVK_GLU_SILU) {
     float s;
     if constexpr (sizeof(T) == 4) s = 1.0f / (1.0f + expf(-g));
     else s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
     a = g * s;
-    d = s * (1.0f + g * (1.0f - s));
+    d = s * (1.0f + b * (1.0f - s));
   } else if (act == SVK_GLU_GELU) {
     const float p = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
     a = g * p;
-    d = p + g * 0.3989422804014327f * expf(-0.5f * g * g);
+    d = p + b * 0.3989422804014327f * expf(-0.5f * b * b);
   } else {
     a = g > 0.f ? g : (g <= 0.f ? 0.f : g);
     d = g > 0.f ? 1.f : 0.f;

@@ -283,6 +283,23 @@ def test_gated_ffn_bwd_values(cuda, dt, act):
         _within(got, ref, tol + u_ * (ref.abs() + tol) + 2.0 ** -25, act)
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_ffn_bwd_kept_gates_that_left_the_range(cuda, dt, act):
+    """Gates kept as infinities: act and act' are 0 below, act' is 1 above; integers elsewhere, so all of it is exact."""
+    ops = _ops()
+    M, H, K = 3, 24, 16
+    x, w = _ints(M, K, dt=dt, seed=1), _ints(2 * H, K, dt=dt, seed=2)
+    dh, u = _ints(M, H, dt=dt, seed=3, top=3), _ints(M, H, dt=dt, seed=4, top=3)
+    g = torch.full((M, H), -float("inf"), device="cuda", dtype=dt)
+    pre = torch.cat([g, u], 1)
+    dx, dw, db = ops.gated_ffn_bwd(x, w, pre, dh, act=act)
+    assert not bool(dx.any()) and not bool(dw.any()) and not bool(db.any())       # NaN.any() is true
+    dx, dw, db = ops.gated_ffn_bwd(x, w, torch.cat([-g, u], 1), dh, act=act)
+    assert torch.equal(db[:H].to(F64), (dh.to(F64) * u.to(F64)).sum(0))
+    assert torch.equal(dw[:H].to(F64), (dh.to(F64) * u.to(F64)).t() @ x.to(F64))
+
+
 def test_gated_ffn_gradient_against_differences(cuda):
     """f32: the derivative of sum(h * dh) along random directions of x, w and the bias, by central differences of the
     forward kernel.  Steps of 2^-6: third-order term ~ 2^-12 of the slope's scale, rounding ~ 2^-24 / 2^-6."""
