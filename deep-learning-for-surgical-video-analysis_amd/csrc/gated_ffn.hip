@@ -290,8 +290,9 @@ __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, con
   }
 }
 
-// rows a workgroup of gated_dpre: 64, fewer where that leaves CUs idle (16: 4 a wave)
-inline int dpre_rows(long m, long h) { return m * h >= 1L << 23 ? 64 : 16; }
+// rows a workgroup of gated_dpre: 64, fewer where that leaves CUs idle (16: 4 a wave), more where the launch would have
+// 2^32 threads
+inline int dpre_rows(long m, long h) { return m >= 1L << 29 ? 1024 : (m * h >= 1L << 23 ? 64 : 16); }
 
 // workspace of the backward pass: [dpre][x padded][w padded][bias partials][slabs of dx][slabs of dW]
 struct BwdWs {

@@ -276,8 +276,11 @@ extern "C" int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long 
     int8_t* q = (int8_t*)Q;
     auto go = [&](auto nch, auto rw) {
       constexpr int RW = decltype(rw)::value;
-      hipLaunchKernelGGL((quant_rows<T, decltype(nch)::value, RW>), dim3((unsigned)((M + 4 * RW - 1) / (4 * RW))),
-                         dim3(256), 0, st, x, ldx, q, ldq, S, M, (int)K);
+      for (long m = 0; m < M; m += 1L << 25) {                  // a launch has under 2^32 threads, 64 a row here
+        const long rows = std::min(M - m, 1L << 25);
+        hipLaunchKernelGGL((quant_rows<T, decltype(nch)::value, RW>), dim3((unsigned)((rows + 4 * RW - 1) / (4 * RW))),
+                           dim3(256), 0, st, x + m * ldx, ldx, q + m * ldq, ldq, S + m, rows, (int)K);
+      }
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;

@@ -156,9 +156,10 @@ extern "C" int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo
                           const void* K, long ldk, long sbk, void* Ko, long ldko, long sbko, int kv_heads, const void* pos,
                           int pos_type, long ldp, long sbp, const double* freqs, int nt, int nh, int nw, int hd, int B, int N,
                           int interleaved, int inverse, void* stream) {
-  const int R = nt + nh + nw;
+  const long Rl = (long)nt + nh + nw;
+  const int R = (int)Rl;
   if (!Q || !Qo || heads <= 0 || kv_heads < 0 || (kv_heads && (!K || !Ko)) || !pos || !freqs || nt < 0 || nh < 0 || nw < 0 ||
-      R < 1 || 2 * (long)R > hd || B < 0 || N < 0 || (pos_type != SVK_POS_I32 && pos_type != SVK_POS_I64 && pos_type != SVK_POS_F32)) {
+      Rl < 1 || 2 * Rl > hd || B < 0 || N < 0 || (pos_type != SVK_POS_I32 && pos_type != SVK_POS_I64 && pos_type != SVK_POS_F32)) {
     set_error("svk_rope3d: bad args");
     return SVK_EINVAL;
   }
@@ -180,7 +181,9 @@ extern "C" int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo
     // about 1024 units (4 a thread) a workgroup, fewer where that would leave CUs idle; the table within 32 KiB of LDS
     const long upt = (long)(heads + kv_heads) * ((hd + V - 1) / V);
     long tpb = std::min<long>(std::max<long>(1, 1024 / upt), std::max<long>(1, a.tokens / 2048));
-    a.tpb = (int)std::max<long>(1, std::min<long>(tpb, 4096 / R));
+    tpb = std::max<long>(1, std::min<long>(tpb, 4096 / R));
+    a.tpb = (int)std::max<long>(tpb, ((long)a.tokens + (1L << 23) - 1) >> 23);   // a launch has under 2^32 threads
+    if ((long)a.tpb * R > 8192) { set_error("svk_rope3d: too many tokens of so many pairs"); return SVK_EUNSUPPORTED; }
     if (pos_type == SVK_POS_I32) return launch<T, int>(a, interleaved, (hipStream_t)stream);
     if (pos_type == SVK_POS_I64) return launch<T, long>(a, interleaved, (hipStream_t)stream);
     return launch<T, float>(a, interleaved, (hipStream_t)stream);

@@ -23,7 +23,7 @@ def _rope(lib, **kw):
 
 
 @pytest.mark.parametrize("kw", [dict(q=None), dict(qo=None), dict(heads=0), dict(k=None), dict(ko=None), dict(kv=-1),
-                                dict(pos=None), dict(freqs=None), dict(nt=-1), dict(nt=0, nh=0, nw=0), dict(nt=3),
+                                dict(pos=None), dict(freqs=None), dict(nt=-1), dict(nt=2 ** 31 - 1, nh=2 ** 31 - 1, nw=4), dict(nt=0, nh=0, nw=0), dict(nt=3),
                                 dict(pt=3), dict(B=-1), dict(N=-1), dict(dt=7)])
 def test_rope3d_refuses(kw):
     lib = _lib()

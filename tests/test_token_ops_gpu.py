@@ -424,6 +424,18 @@ def test_quant_rows(cuda, dt, M, K):
     _within(q.to(F64) * s.to(F64)[:, None], x.to(F64), (0.5 + 2.0 ** -15) * s.to(F64)[:, None].expand(M, K) + 1e-30, "values")
 
 
+def test_quant_rows_more_rows_than_one_launch(cuda):
+    """2^26 rows, 64 threads each, are 2^32 threads."""
+    ops = _ops()
+    M = (1 << 26) + 5
+    x = torch.zeros(M, 4, device="cuda", dtype=torch.float16)
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, M - 1], device="cuda")
+    x[at] = _ints(len(at), 4, dt=torch.float16, seed=1, top=9)
+    q, s = ops.quant_rows(x)
+    q2, s2 = ops.quant_rows(x[at])
+    assert torch.equal(q[at], q2) and torch.equal(s[at], s2) and int((s != 0).sum()) == int((s2 != 0).sum())
+
+
 def test_quant_rows_ties_and_scales_of_all_sizes(cuda):
     """Quotients on and next to half integers (16-bit values divide to exact ties often), and scales from subnormal to
     1e36: still the correctly rounded quotient, rounded."""
