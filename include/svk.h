@@ -606,15 +606,16 @@ int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo, long ldqo
 
 /* Gated feed-forward block (csrc/gated_ffn.hip): Hout = act(X Wg^T + bg) * (X Wu^T + bu), one kernel.  X [M, K], W =
  * [Wg; Wu] [2H, K], bias = [bg; bu] [2H] f32 or NULL, Hout [M, H]; act = SVK_GLU_*.  pre (NULL, or [M, 2H] contiguous):
- * receives the two projections rounded to dtype, for svk_gated_ffn_bwd.  ws: svk_gated_ffn_workspace bytes (0 where the
- * rows of X and W are whole 16-byte pieces; 16-byte aligned otherwise). */
+ * receives the two projections rounded to dtype, for svk_gated_ffn_bwd (one that leaves f16's range is kept as an
+ * infinity).  ws: svk_gated_ffn_workspace bytes, 16-byte aligned (0 up to 64 tokens, and where the rows of X and W are whole
+ * aligned 16-byte pieces).  W under 4 GiB.  Outputs overlap no input. */
 long svk_gated_ffn_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K);
 int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, long ldw, const float* bias, void* Hout, long ldh,
                   void* pre, long M, long H, long K, int act, void* ws, long ws_bytes, void* stream);
 /* Its backward pass from dH [M, H] and pre: with dP = [dH * u * act'(g) | dH * act(g)] (rounded to dtype once)
  * dX [M, K] = dP W, dW [2H, K] contiguous = dP^T X, db [2H] f32 = column sums of dP before its rounding.  Each of dX, dW,
- * db may be NULL; they are written, not added to, in the same order of summation on every run.  ws:
- * svk_gated_ffn_bwd_workspace bytes, 16-byte aligned. */
+ * db may be NULL; they are written, not added to, in the same order of summation on every run, and overlap no
+ * input.  M = 0 writes zeros to dW and db.  ws: svk_gated_ffn_bwd_workspace bytes, 16-byte aligned. */
 long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K,
                                  int want_dx, int want_dw, int want_db);
 int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH,
@@ -625,8 +626,9 @@ int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ld
  * to the nearest integer (ties to even); a row of zeros has S = 0 and codes 0, a row with an infinity or a NaN S = NaN
  * and codes 0.  For weights [N, K] the same gives the scale of each output channel.
  * svk_gemm_i8: Y = act((A W^T as integers) * sa[m] * sw[n] + bias[n]) + R, A [M, K] and W [N, K] int8, sa [M], sw [N],
- * bias [N] f32 (or NULL), R (or NULL) and Y [M, N] in dtype.  The integer sums are exact: K <= 131071.  ws:
- * svk_gemm_i8_workspace bytes (0 where the rows of A and W are whole 16-byte pieces; 16-byte aligned otherwise). */
+ * bias [N] f32 (or NULL), R (or NULL) and Y [M, N] in dtype.  The integer sums are exact: K <= 131071.  W under 4 GiB.  Y may
+ * be R itself (same stride), and overlaps no other input.  ws: svk_gemm_i8_workspace bytes, 16-byte aligned (0 up to 64
+ * tokens, and where W's rows are whole aligned 16-byte pieces and A's are aligned and that far apart). */
 int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long ldq, float* S, long M, long K, void* stream);
 long svk_gemm_i8_workspace(const void* A, long lda, const void* W, long ldw, long M, long N, long K);
 int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, const void* W, long ldw, const float* sw,

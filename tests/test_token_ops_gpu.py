@@ -779,3 +779,63 @@ def test_results_do_not_change_from_run_to_run(cuda):
     for _ in range(3):
         for a, b in zip(first, ops.gated_ffn_bwd(x, w, pre, h)):
             assert torch.equal(a, b)
+
+
+def test_operands_past_32_bits(cuda):
+    """Rows, results and gradients that lie more than 4 GiB behind their first: sparse integers, so all of it is exact."""
+    ops = _ops()
+    M, K, H, dt = (1 << 20) + 70, 2112, 1056, torch.bfloat16
+    at = torch.tensor([0, 77, 1 << 19, (1 << 20) - 1, M - 1], device="cuda")
+    x = torch.zeros(M, K, device="cuda", dtype=dt)
+    x[at] = _ints(len(at), K, dt=dt, seed=1)
+    w = _ints(2 * H, K, dt=dt, seed=2)
+    h, pre = ops.gated_ffn(x, w, act="relu", save=True)                 # x, pre 4.4 GB
+    assert torch.equal(h[at], ops.gated_ffn(x[at], w, act="relu")) and int(h.any(1).sum()) <= len(at)
+    dh = torch.zeros(M, H, device="cuda", dtype=dt)
+    dh[at] = _ints(len(at), H, dt=dt, seed=3)
+    got, ref = ops.gated_ffn_bwd(x, w, pre, dh, act="relu"), ops.gated_ffn_bwd(x[at], w, pre[at], dh[at], act="relu")
+    assert torch.equal(got[0][at], ref[0]) and int(got[0].any(1).sum()) <= len(at)
+    assert torch.equal(got[2], ref[2])
+    # dW in either order of its few terms: f32 sums of at most five 16-bit products, each partial sum rounded, then once
+    tol = pre[at].float().abs().amax() * 5 * 4 * 2.0 ** -24
+    _within(got[1], ref[1].to(F64), tol + 2 * U[dt] * ref[1].to(F64).abs(), "dW")
+    del got, h, pre, dh
+    q = x.view(M, K)[None]
+    pos = torch.zeros(M, 3, device="cuda", dtype=torch.int32)
+    pos[at] = torch.tensor([3, 5, 7], device="cuda", dtype=torch.int32)
+    freqs = ops.rope3d_freqs((4, 4, 4))
+    y = ops.rope3d(q, None, pos, freqs, (4, 4, 4), K // 32)[0]
+    assert torch.equal(y[0, at], ops.rope3d(q[:, at], None, pos[at], freqs, (4, 4, 4), K // 32)[0][0])
+    assert int(y[0].any(1).sum()) <= len(at)
+    del y
+    a = torch.zeros(2 * M, K, device="cuda", dtype=torch.int8)
+    a[2 * at] = _codes(len(at), K, 5)
+    b, s = _codes(64, K, 6), torch.ones(2 * M, device="cuda")
+    y = ops.gemm_i8(a, s, b, s[:64], dtype=torch.float32)
+    assert torch.equal(y[2 * at], ops.gemm_i8(a[2 * at], s[:5], b, s[:64], dtype=torch.float32))
+    assert int(y.any(1).sum()) <= len(at)
+
+
+@pytest.mark.parametrize("M", [3, 70, 300])
+def test_weights_of_almost_4_gib(cuda, M):
+    """The largest weights that are taken (the offset of the last row is just under 2^32), all of it exact."""
+    ops = _ops()
+    N, K = (1 << 20) + 4096 + 40, 4064
+    assert N * K < 1 << 32 <= (N + 8192) * K
+    w = torch.zeros(N, K, device="cuda", dtype=torch.int8)
+    at = torch.tensor([0, 5000, 1 << 19, (1 << 20) + 1, N - 2, N - 1], device="cuda")
+    w[at] = _codes(len(at), K, 1)
+    a, one = _codes(M, K, 2), torch.ones(N, device="cuda")
+    y = ops.gemm_i8(a, one[:M], w, one, dtype=torch.float32)
+    ref = (a.cpu().double() @ w[at].cpu().double().t()).float().cuda()
+    assert torch.equal(y[:, at], ref) and int(y.any(0).sum()) <= len(at)
+    del w, y
+    H, K = N // 2, 2032
+    w = torch.zeros(2 * H, K, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 5000, 1 << 18, H - 2, H - 1], device="cuda")
+    w[at], w[H + at] = (_ints(len(at), K, dt=torch.bfloat16, seed=s) for s in (3, 4))
+    x = _ints(M, K, dt=torch.bfloat16, seed=5)
+    h = ops.gated_ffn(x, w, act="relu")
+    g, u = ((x.cpu().double() @ w[i].cpu().double().t()) for i in (at, H + at))
+    # the product of two integers under 2^11 is exact in f32
+    assert torch.equal(h[:, at], (g.relu() * u).to(torch.bfloat16).cuda()) and int(h.any(0).sum()) <= len(at)
