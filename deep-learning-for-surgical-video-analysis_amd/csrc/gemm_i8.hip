@@ -1,7 +1,7 @@
 // Matrix product in 8-bit integers with a scale for each token and each output channel (svk_gemm_i8), and the
 // quantisation of token rows that feeds it (svk_quant_rows):
 //
-//   s[m] = max_k |x[m, k]| / 127,  q[m, k] = round(x[m, k] / s[m])            (ties to even; a row of zeros: s = 0, q = 0)
+//   s[m] = max_k |x[m, k]| (1 / 127),  q[m, k] = round(x[m, k] / s[m])        (ties to even; a row of zeros: s = 0, q = 0)
 //   C[m, n] = act((sum_k qa[m, k] qw[n, k]) sa[m] sw[n] + bias[n]) + R[m, n]
 //
 // The integer sums are exact (int32: K <= 131071, 2^31 / 128^2 less one); everything behind them is f32, rounded once.
@@ -45,10 +45,12 @@ __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, long 
   if (row0 >= M) return;
   constexpr int W = 2 * sizeof(T);                              // words of 8 values
   float s, inv;
-  // the scale from the largest magnitude, and its reciprocal; 0 where the scale is so small that the residual would
+  // the scale from the largest magnitude (times the f32 1 / 127: what torch's x.abs().amax(-1) / 127 is on the GPU, so the
+  // codes are those of that expression; a true division differs by a step in one row of 20, and with it decided 1 of 14000
+  // codes of bf16 tokens the other way), and its reciprocal; 0 where the scale is so small that the residual would
   // underflow (then codes come from the division), or is no finite number, or 0 (codes of 0)
   auto scale = [&](long row, float top) {
-    s = top < INFINITY ? top / 127.f : NAN;
+    s = top < INFINITY ? top * (1.f / 127.f) : NAN;
     inv = s >= 1e-30f ? 1.f / s : 0.f;
     if (lane == 0) S[row] = s;
   };

@@ -1742,8 +1742,9 @@ def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
 
 
 def quant_rows(x):
-    """(codes int8 [..., K], scale float32 [...]) with x ~ codes * scale: scale = max |row| / 127, codes
-    x / scale rounded to the nearest, ties to even (svk_quant_rows).  Tokens before ``gemm_i8``; a weight [N, K] once, when it is loaded.  Rows of
+    """(codes int8 [..., K], scale float32 [...]) with x ~ codes * scale: scale = max |row| * (1 / 127) in
+    float32 (torch's ``x.float().abs().amax(-1) / 127`` on the GPU), codes x / scale rounded to the nearest, ties to even
+    (svk_quant_rows).  Tokens before ``gemm_i8``; a weight [N, K] once, when it is loaded.  Rows of
     the codes are a multiple of 16 bytes apart (a view of a padded buffer where K % 16 != 0)."""
     dt, dev = _code(x, "quant_rows", "x")
     M, K, ldx = _token_rows(x, "quant_rows", "x")

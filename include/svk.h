@@ -622,8 +622,8 @@ int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ld
                       long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K, int act, void* ws,
                       long ws_bytes, void* stream);
 
-/* 8-bit integer products (csrc/gemm_i8.hip).  svk_quant_rows: S[m] = max |X[m, :]| / 127, Q[m, k] = X[m, k] / S[m] rounded
- * to the nearest integer (ties to even); a row of zeros has S = 0 and codes 0, a row with an infinity or a NaN S = NaN
+/* 8-bit integer products (csrc/gemm_i8.hip).  svk_quant_rows: S[m] = max |X[m, :]| * (1 / 127) in f32, Q[m, k] =
+ * X[m, k] / S[m] rounded to the nearest integer (ties to even); a row of zeros has S = 0 and codes 0, a row with an infinity or a NaN S = NaN
  * and codes 0.  For weights [N, K] the same gives the scale of each output channel.
  * svk_gemm_i8: Y = act((A W^T as integers) * sa[m] * sw[n] + bias[n]) + R, A [M, K] and W [N, K] int8, sa [M], sw [N],
  * bias [N] f32 (or NULL), R (or NULL) and Y [M, N] in dtype.  The integer sums are exact: K <= 131071.  W under 4 GiB.  Y may

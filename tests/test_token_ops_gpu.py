@@ -406,22 +406,34 @@ def test_gated_ffn_refusals(cuda):
 
 # ---------------------------------------------------------------- 8-bit integer products
 
+_127TH = torch.tensor(1 / 127, dtype=torch.float32)
+
+
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("M,K", [(1, 1), (5, 7), (3, 64), (130, 333), (9, 512), (4, 520), (2, 1024), (3, 2048), (2, 4096), (2, 5000), (2, 4099)])
 def test_quant_rows(cuda, dt, M, K):
-    """The scale and x / scale are f32 divisions, correctly rounded on both sides: equal bit for bit."""
+    """The scale is one f32 product and x / scale an f32 division, correctly rounded on both sides: equal bit for bit."""
     ops = _ops()
     x = _rand(M, K, dt=dt, seed=1, scale=3.0)
     if M > 1:
         x[1] = 0
     q, s = ops.quant_rows(x)
     xf = x.float().cpu()
-    want_s = xf.abs().amax(1) / 127
+    want_s = xf.abs().amax(1) * _127TH
     want_q = torch.where(want_s[:, None] > 0, torch.round(xf / want_s[:, None]), torch.zeros_like(xf))
     assert q.shape == (M, K) and s.shape == (M,) and q.stride(0) % 16 == 0
     assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q.to(torch.int8))
     # a row's values are kept to half a step of its scale
     _within(q.to(F64) * s.to(F64)[:, None], x.to(F64), (0.5 + 2.0 ** -15) * s.to(F64)[:, None].expand(M, K) + 1e-30, "values")
+
+
+@pytest.mark.parametrize("dt", DTS)
+def test_quant_rows_has_the_codes_of_the_torch_expression(cuda, dt):
+    ops = _ops()
+    x = _rand(2000, 1056, dt=dt, seed=7)
+    s = x.float().abs().amax(1) / 127
+    q, sc = ops.quant_rows(x)
+    assert torch.equal(sc, s) and torch.equal(q.float(), torch.round(x.float() / s[:, None]))
 
 
 def test_quant_rows_more_rows_than_one_launch(cuda):
@@ -446,7 +458,7 @@ def test_quant_rows_ties_and_scales_of_all_sizes(cuda):
     rows = [x * 2.0 ** e * f for e in (-140, -126, -100, -60, 0, 60, 110) for f in (1.0, 1.1, 1.9999999)]
     rows += [torch.randn(len(x), generator=g).half().float() * 2.0 ** -e for e in range(12)]
     x = torch.stack(rows)
-    s = x.abs().amax(1, keepdim=True) / 127
+    s = x.abs().amax(1, keepdim=True) * _127TH
     want = torch.where(s > 0, torch.round(x / s), torch.zeros_like(x)).clamp(-127, 127)
     q, sc = ops.quant_rows(x.cuda())
     fine = s[:, 0] >= 2.0 ** -126                 # a subnormal scale is a rough number, but the same on both sides
@@ -454,7 +466,7 @@ def test_quant_rows_ties_and_scales_of_all_sizes(cuda):
     assert int(q.abs().max()) <= 127
     for dt in (torch.float16, torch.bfloat16):
         y = (torch.randint(-2000, 2001, (500, 256), generator=g).float() / 64).to(dt)
-        s = y.float().abs().amax(1, keepdim=True) / 127
+        s = y.float().abs().amax(1, keepdim=True) * _127TH
         assert torch.equal(ops.quant_rows(y.cuda())[0].cpu().float(), torch.round(y.float() / s))
 
 
