@@ -168,6 +168,15 @@ extern "C" int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo
     return SVK_EUNSUPPORTED;
   }
   if (B == 0 || N == 0) return SVK_OK;
+  // in place with the same strides only, and neither output in the other's input (read by other threads meanwhile)
+  auto moved = [&](const void* in, long ld, long sb, const void* out, long ldo, long sbo) {
+    return in == out && ((N > 1 && ld != ldo) || (B > 1 && sb != sbo));
+  };
+  if (moved(Q, ldq, sbq, Qo, ldqo, sbqo) ||
+      (kv_heads && (Qo == K || Ko == Q || Qo == Ko || moved(K, ldk, sbk, Ko, ldko, sbko)))) {
+    set_error("svk_rope3d: an output overlaps an input or the other output");
+    return SVK_EINVAL;
+  }
   SVK_DISPATCH_DTYPE(dtype, T, {
     RopeArgs a{};
     a.q = Map{(const char*)Q, (char*)Qo, ldq, sbq, ldqo, sbqo, heads};

@@ -1553,9 +1553,9 @@ def _vector(t, n, dev, fn, name):
         raise _lib.SvkError(f"svk.{fn}: {name} must be {n} contiguous float32 values, got {tuple(t.shape)}")
 
 
-def _apart(a, b):
-    """False where writing ``a`` may change ``b``: their memory meets, and they are not the same elements in the same
-    order, nor two column ranges of one buffer's rows."""
+def _apart(a, b, same=True):
+    """False where writing ``a`` may change ``b``: their memory meets, and they are neither two column ranges of one
+    buffer's rows nor (``same``: where every value of b is read by who writes it) the same elements in the same order."""
     if a is None or b is None or a.numel() == 0 or b.numel() == 0:
         return True
     ea, eb = a.element_size(), b.element_size()
@@ -1565,7 +1565,7 @@ def _apart(a, b):
     if ea != eb:
         return False
     if a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride():
-        return True
+        return same
     if a.dim() == b.dim() and a.shape[:-1] == b.shape[:-1] and a.stride() == b.stride() and a.dim() > 1:
         ld = min((s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1), default=0)
         if ld and all(s % ld == 0 for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1):
@@ -1586,8 +1586,9 @@ def rope3d_freqs(sections, base=10000.0, shared=False, device="cuda"):
     return torch.pow(torch.tensor(float(base), dtype=torch.float64), -e).to(device)
 
 
-def _rope_out(q, k, out):
-    """The given outputs of rope3d, checked."""
+def _rope_out(q, k, out, *tables):
+    """The given outputs of rope3d, checked: each may be its own input, and meets neither the other input, nor the other
+    output, nor ``tables`` (positions, frequencies): other threads read those while it is written."""
     qo, ko = out
     if (ko is None) != (k is None):
         raise _lib.SvkError("svk.rope3d: out must be (q', k') like (q, k)")
@@ -1601,8 +1602,8 @@ def _rope_out(q, k, out):
         sb, sn, sc = o.stride()
         if (width > 1 and sc != 1) or (N > 1 and sn < width) or (B > 1 and sb < (sn * (N - 1) if N > 1 else 0) + width):
             raise _lib.SvkError("svk.rope3d: out rows overlap or lack unit channel stride")
-    if not (_apart(qo, q) and _apart(qo, k) and _apart(ko, k) and _apart(ko, q) and _apart(qo, ko)) or \
-            (ko is not None and qo.data_ptr() == ko.data_ptr() and qo.numel()):
+    if not (_apart(qo, q) and _apart(ko, k) and _apart(qo, k, same=False) and _apart(ko, q, same=False) and
+            _apart(qo, ko, same=False) and all(_apart(o, t, same=False) for o in (qo, ko) for t in tables)):
         raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
     return qo, ko
 
@@ -1613,7 +1614,7 @@ def rope3d(q, k, pos, freqs, sections, heads, kv_heads=None, interleaved=False, 
     q [B, N, heads * hd], k [B, N, kv_heads * hd] or None (any row / batch strides, unit channel stride); pos [N, 3] or
     [B, N, 3] int32 / int64 / float32; sections = pairs of the three axes, in this order, 2 * sum <= hd; freqs float64
     [sum(sections)] (rope3d_freqs).  ``inverse`` turns back: the gradient of the rotation.  ``out`` = (q', k') to write,
-    which may be (q, k)."""
+    which may be (q, k); q' must not meet k, nor k' q."""
     dt, dev = _code(q, "rope3d", "q")
     shape = q.shape
     if len(shape) != 3 or heads < 1 or shape[2] % heads or shape[2] == 0:
@@ -1654,7 +1655,7 @@ def rope3d(q, k, pos, freqs, sections, heads, kv_heads=None, interleaved=False, 
             ko = torch.empty_like(k) if k.is_contiguous() else torch.empty(k.shape, device=q.device, dtype=q.dtype)
             kos = (N * kv_heads * hd, kv_heads * hd)
     else:
-        qo, ko = _rope_out(q, k, out)
+        qo, ko = _rope_out(q, k, out, pos, freqs)
         qos = qo.stride()
         kos = None if ko is None else ko.stride()
     if B * N:

@@ -597,7 +597,8 @@ int svk_pack_transpose(int dtype, const void* tiles, int ntiles, const float* sr
  * -th, which is the gradient.  Pairs are channels (i, i + R) of a head, or (2i, 2i + 1) if interleaved; channels 2R ..
  * hd - 1 are copied.  Q / K [B, N, heads * hd] with unit channel stride, ld* values between tokens and sb* between
  * batches; kv_heads = 0: no K.  pos [B, N, 3] of pos_type (SVK_POS_*), unit stride in the last dim, sbp = 0: the same
- * positions for every batch.  freqs [R] f64, radians a step.  Outputs may be the inputs themselves (same strides).
+ * positions for every batch.  freqs [R] f64, radians a step.  Qo may be Q and Ko may be K (same strides); neither
+ * overlaps anything else.
  * Angles are formed in 64 bits; a position that is not finite gives NaN in the channels that follow its axis. */
 int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo, long ldqo, long sbqo, int heads, const void* K,
                long ldk, long sbk, void* Ko, long ldko, long sbko, int kv_heads, const void* pos, int pos_type, long ldp,

@@ -181,3 +181,36 @@ def test_apart_views():
     assert not ops._apart(q, b[..., 5:15]) and not ops._apart(b[..., 5:15], q)
     assert not ops._apart(b[:3], b[1:]) and not ops._apart(b[..., 25:], b.flatten()[5:])
     assert not ops._apart(q, b.view(torch.float16)[..., :10])
+
+
+def test_rope3d_outputs_in_the_other_input_or_in_the_tables():
+    """An output may be its own input only: what it wrote elsewhere would be read as the other input by other threads."""
+    import svk
+    from svk import ops
+    t = torch.zeros(2, 5, 64)
+    q, k, new = t[..., :32], t[..., 32:], torch.zeros(2, 5, 32)
+    pos = torch.zeros(5, 3)
+    assert ops._rope_out(q, k, (q, k), pos)[0] is q                    # in place, packed
+    ops._rope_out(q, k, (new, new.clone()), pos)
+    ops._rope_out(q, q, (new, new.clone()), pos)                       # the inputs may be one
+    ops._rope_out(q, None, (q, None), pos)
+    for a in ((q, k, (k, q)), (q, k, (k, new)), (q, k, (new, q)), (q, q, (q, new)), (q, q, (new, q)), (q, k, (new, new)),
+              (q, k[..., :16], (k, new[..., :16])), (q, k, (q, k), q[0, :, :3]),
+              (q, k, (q, k), pos, t.view(torch.float64).flatten()[-8:])):
+        with pytest.raises(svk.SvkError, match="overlaps"):
+            ops._rope_out(*a)
+
+
+B = 0x40000000       # another made-up address
+
+
+@pytest.mark.parametrize("kw", [dict(qo=B, ko=B), dict(q=B, k=A, qo=A, ko=2 * B), dict(q=A, k=B, qo=2 * B, ko=A),
+                                dict(q=A, k=A, qo=A, ko=B), dict(q=A, k=B, qo=B, ko=A),
+                                dict(q=A, qo=A, k=B, ko=2 * B, ldqo=32), dict(q=A, qo=2 * B, k=B, ko=B, sbko=64)])
+def test_rope3d_entry_refuses_outputs_that_meet(kw):
+    lib = _lib()
+    a = dict(q=A, qo=2 * B, k=B, ko=3 * B, ldqo=16, sbko=32)
+    a.update(kw)
+    rc = lib.svk_rope3d(0, a["q"], 16, 64, a["qo"], a["ldqo"], 64, 2, a["k"], 8, 32, a["ko"], 8, a["sbko"], 1, 4 * B, 0, 3, 0, 5 * B,
+                        2, 1, 1, 8, 2, 4, 0, 0, None)
+    assert rc == -1 and b"overlaps" in lib.svk_last_error()
