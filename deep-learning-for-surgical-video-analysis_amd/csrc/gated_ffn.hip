@@ -265,7 +265,11 @@ __global__ __launch_bounds__(256) void gated_dpre(const T* __restrict__ pre, con
       for (int e = 0; e < V; ++e) {
         float a, da;
         glu_grad<T>(to_f(g[e]), act, a, da);
-        const float dg = to_f(d[e]) * to_f(u[e]) * da, du = to_f(d[e]) * a;
+        // a dh of 0, and an act' of 0 under a finite dh, win over an infinity (a projection kept past f16's range, whose
+        // f32 value the forward pass multiplied by 0; dh u past f32's range); NaN passes
+        const float f = to_f(d[e]), v = to_f(u[e]);
+        const bool zero = f == 0.f ? da == da : da == 0.f && fabsf(f) < INFINITY;
+        const float dg = zero && v == v ? 0.f : f * v * da, du = f == 0.f && a == a ? 0.f : f * a;
         og[e] = from_f<T>(dg);
         ou[e] = from_f<T>(du);
         sg[e] += dg;

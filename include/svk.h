@@ -608,8 +608,9 @@ int svk_rope3d(int dtype, const void* Q, long ldq, long sbq, void* Qo, long ldqo
 /* Gated feed-forward block (csrc/gated_ffn.hip): Hout = act(X Wg^T + bg) * (X Wu^T + bu), one kernel.  X [M, K], W =
  * [Wg; Wu] [2H, K], bias = [bg; bu] [2H] f32 or NULL, Hout [M, H]; act = SVK_GLU_*.  pre (NULL, or [M, 2H] contiguous):
  * receives the two projections rounded to dtype, for svk_gated_ffn_bwd (one that leaves f16's range is kept as an
- * infinity).  ws: svk_gated_ffn_workspace bytes, 16-byte aligned (0 up to 64 tokens, and where the rows of X and W are whole
- * aligned 16-byte pieces).  W under 4 GiB.  Outputs overlap no input. */
+ * infinity; there a zero dH or act' gives 0 with it, as in the forward pass).  ws: svk_gated_ffn_workspace bytes, 16-byte
+ * aligned (0 up to 64 tokens, and where the rows of X and W are whole aligned 16-byte pieces).  W under 4 GiB.  Outputs
+ * overlap no input. */
 long svk_gated_ffn_workspace(int dtype, const void* X, long ldx, const void* W, long ldw, long M, long H, long K);
 int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, long ldw, const float* bias, void* Hout, long ldh,
                   void* pre, long M, long H, long K, int act, void* ws, long ws_bytes, void* stream);

@@ -300,6 +300,47 @@ def test_gated_ffn_bwd_kept_gates_that_left_the_range(cuda, dt, act):
     assert torch.equal(dw[:H].to(F64), (dh.to(F64) * u.to(F64)).t() @ x.to(F64))
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_ffn_bwd_kept_projections_that_left_the_range_behind_zeros(cuda, dt, act):
+    """Projections kept as infinities (f16's range) where the other factor is zero: the forward pass held them in f32
+    and gave 0, so does the gradient.  All of it is exact."""
+    ops = _ops()
+    inf = float("inf")
+    M, H, K = 3, 24, 16
+    x, w = _ints(M, K, dt=dt, seed=1), _ints(2 * H, K, dt=dt, seed=2)
+    dh = _ints(M, H, dt=dt, seed=3, top=3)
+    big = torch.full((M, H), inf, device="cuda", dtype=dt)
+    big[:, ::2] = -inf
+    shut = torch.full((M, H), -1e4, device="cuda", dtype=dt)           # act and act' are zeros of f32
+    none = torch.zeros(M, H, device="cuda", dtype=dt)
+    for pre, d in ((torch.cat([shut, big], 1), dh), (torch.cat([big, big], 1), none), (torch.cat([big.abs(), big], 1), none)):
+        for t in ops.gated_ffn_bwd(x, w, pre, d, act=act):
+            assert not bool(t.any())                                   # NaN.any() is true
+    # open gates: the infinities pass where dh is not zero, and nowhere else
+    one = torch.ones(1, K, device="cuda", dtype=dt)
+    d = dh[:1]
+    dx, dw, db = ops.gated_ffn_bwd(one, w, torch.cat([big[:1].abs(), big[:1].abs()], 1), d, act=act)
+    want = torch.where(d[0] == 0, 0.0, d[0].float() * inf)
+    assert torch.equal(db, torch.cat([want, want])) and torch.equal(dw.float(), db[:, None].expand(2 * H, K))
+    # NaN is never hidden, nor an infinite dh
+    nan = torch.full((1, H), float("nan"), device="cuda", dtype=dt)
+    for g, u, d in ((shut[:1], nan, none[:1]), (nan, shut[:1], none[:1]), (shut[:1], shut[:1], big[:1])):
+        assert bool(ops.gated_ffn_bwd(one, w, torch.cat([g, u], 1), d, act=act)[0].isnan().all())
+
+
+def test_gated_ffn_bwd_products_past_the_range_behind_closed_gates(cuda):
+    """dh * u leaves f32's range, act' is zero: the gradient of the gate is zero."""
+    ops = _ops()
+    for dt in (torch.float32, torch.bfloat16):
+        x, w = _ints(2, 16, dt=dt, seed=1), _ints(16, 16, dt=dt, seed=2)
+        pre = torch.full((2, 16), 2.0 ** 100, device="cuda", dtype=dt)
+        pre[:, :8] = -1e4
+        for act in ("silu", "gelu", "relu"):
+            for t in ops.gated_ffn_bwd(x, w, pre, pre[:, 8:].contiguous(), act=act):
+                assert not bool(t.any())
+
+
 def test_gated_ffn_gradient_against_differences(cuda):
     """f32: the derivative of sum(h * dh) along random directions of x, w and the bias, by central differences of the
     forward kernel.  Steps of 2^-6: third-order term ~ 2^-12 of the slope's scale, rounding ~ 2^-24 / 2^-6."""
