@@ -1485,8 +1485,8 @@ def mstcn_bwd_floats(T, F):
 GLU_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 _POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _FEW = 64          # tokens up to which the few-token kernels run: they read rows of any alignment and take no workspace
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # absent from a torch without GPU support
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _code(t, fn, name):

@@ -214,3 +214,25 @@ def test_rope3d_entry_refuses_outputs_that_meet(kw):
     rc = lib.svk_rope3d(0, a["q"], 16, 64, a["qo"], a["ldqo"], 64, 2, a["k"], 8, 32, a["ko"], 8, a["sbko"], 1, 4 * B, 0, 3, 0, 5 * B,
                         2, 1, 1, 8, 2, 4, 0, 0, None)
     assert rc == -1 and b"overlaps" in lib.svk_last_error()
+
+
+def test_import_on_a_torch_without_gpu_bindings():
+    """A build of torch without GPU support has no raw-stream query; the package imports, and its operators refuse."""
+    import os
+    import subprocess
+    import sys
+    import svk
+    code = """
+import torch
+for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, n):
+        delattr(torch._C, n)
+import svk
+try:
+    svk.ops.quant_rows(torch.zeros(2, 8))
+except svk.SvkError as e:
+    print("refused:", e)
+"""
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(svk.__file__))))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "no CPU path" in r.stdout, r.stderr
