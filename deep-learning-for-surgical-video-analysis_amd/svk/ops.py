@@ -1598,9 +1598,11 @@ def _rope_out(q, k, out, *tables):
         _like(o, q.dtype, q.get_device(), "rope3d", "out")
         if o.shape != t.shape:
             raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
-        B, N, width = t.shape
-        sb, sn, sc = o.stride()
-        if (width > 1 and sc != 1) or (N > 1 and sn < width) or (B > 1 and sb < (sn * (N - 1) if N > 1 else 0) + width):
+        width, run = t.shape[2], t.shape[2]
+        good = width == 1 or o.stride(2) == 1
+        for s, n in sorted((o.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1):       # either may be the outer dim
+            good, run = good and s >= run, s * (n - 1) + width
+        if not good:
             raise _lib.SvkError("svk.rope3d: out rows overlap or lack unit channel stride")
     if not (_apart(qo, q) and _apart(ko, k) and _apart(qo, k, same=False) and _apart(ko, q, same=False) and
             _apart(qo, ko, same=False) and all(_apart(o, t, same=False) for o in (qo, ko) for t in tables)):

@@ -236,3 +236,16 @@ except svk.SvkError as e:
     env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(svk.__file__))))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
     assert r.returncode == 0 and "no CPU path" in r.stdout, r.stderr
+
+
+def test_rope3d_outputs_of_either_order_of_batch_and_time():
+    import svk
+    from svk import ops
+    qkv = torch.zeros(5, 2, 96).transpose(0, 1)                        # tokens outside, batches inside
+    q, k = qkv[..., :32], qkv[..., 32:64]
+    assert ops._rope_out(q, k, (q, k))[1] is k
+    ops._rope_out(q, k, (torch.zeros(2, 5, 32), torch.zeros(5, 2, 32).transpose(0, 1)))
+    flat = torch.zeros(1000)
+    for bad in ((40, 16, 1), (16, 40, 1), (31, 62, 1), (160, 31, 1), (100, 32, 1), (32, 40, 1), (0, 32, 1), (32, 0, 1), (200, 40, 2)):
+        with pytest.raises(svk.SvkError, match="rows overlap"):
+            ops._rope_out(q, None, (flat.as_strided((2, 5, 32), bad), None))

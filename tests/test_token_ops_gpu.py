@@ -138,6 +138,23 @@ def test_rope3d_strided_packed_in_place(cuda, dt):
     assert z.shape == (0, N, C)
 
 
+@pytest.mark.parametrize("dt", DTS)
+def test_rope3d_time_major_in_place(cuda, dt):
+    """Tokens outside, batches inside (a stream appends a token of every video): turned in place, packed."""
+    ops = _ops()
+    B, N, h, hd, sec = 3, 21, 4, 32, (6, 5, 5)
+    C = h * hd
+    qkv = _rand(N, B, 3 * C, dt=dt, seed=9).transpose(0, 1)
+    q, k, v = qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:]
+    pos = torch.randint(0, 99, (B, N, 3), generator=torch.Generator().manual_seed(1), dtype=torch.int32).cuda()
+    f = ops.rope3d_freqs(sec)
+    want, keep = ops.rope3d(q.contiguous(), k.contiguous(), pos, f, sec, h), v.clone()
+    out = torch.zeros(N, B, C, device="cuda", dtype=dt).transpose(0, 1)
+    assert torch.equal(ops.rope3d(q, None, pos, f, sec, h, out=(out, None))[0], want[0])
+    ops.rope3d(q, k, pos, f, sec, h, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, keep)
+
+
 def test_rope3d_positions_that_are_not_finite(cuda):
     ops = _ops()
     q = torch.ones(1, 2, 8, device="cuda")
