@@ -322,6 +322,10 @@ struct BwdWs {
   }
 };
 
+// (a row that is padded to whole 16-byte pieces has as many stages)
+template <typename T>
+inline Plan forward_plan(long M, long H, long K) { return plan_tiles<T>(M, 2 * H, stages<T>(K), 1); }
+
 static bool bad_dims(long M, long H, long K) {
   // 32-bit row and column counts inside a kernel; 65535 column blocks of gated_dpre
   return M < 0 || H <= 0 || K <= 0 || M > 0x7fffff00L || H > 4000000L || K > 0x1fffff00L;
@@ -343,6 +347,20 @@ extern "C" long svk_gated_ffn_workspace(int dtype, const void* X, long ldx, cons
   if (!es || bad_dims(M, H, K) || M <= SKINNY_M) return 0;
   const long ldk = up16(K * es);
   return (rows_ok(X, ldx, K, es) ? 0 : M * ldk) + (rows_ok(W, ldw, K, es) ? 0 : 2 * H * ldk);
+}
+
+extern "C" int svk_gated_ffn_plan(int dtype, int product, long M, long H, long K, long* plan) {
+  const long es = es_of(dtype);
+  if (!es || bad_dims(M, H, K) || M == 0 || product < 0 || product > 2 || !plan) { set_error("svk_gated_ffn_plan: bad args"); return SVK_EINVAL; }
+  if (product == 0) {
+    if (M <= SKINNY_M) tell_few(M, plan);
+    else tell(es == 4 ? forward_plan<float>(M, H, K) : forward_plan<bf16>(M, H, K), M, plan);
+    return SVK_OK;
+  }
+  const BwdWs ws(es, M, H, K, false, false, product == 1, product == 2);
+  if (product == 1) tell(ws.px, M, plan);
+  else tell(ws.pw, 2 * H, plan);
+  return SVK_OK;
 }
 
 extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, long ldw, const float* bias, void* Hout,
@@ -386,7 +404,7 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
     p.abytes = (M - 1) * p.lda + p.K * es;
     p.bbytes = (2 * H - 1) * p.ldb + p.K * es;
     p.nk = stages<T>(p.K);
-    const Plan plan = plan_tiles<T>(M, 2 * H, p.nk, 1);
+    const Plan plan = forward_plan<T>(M, H, K);
     auto run = [&](auto act_c) {
       GateEpi<T, decltype(act_c)::value> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0, past};
       return launch_plan<T, false, false>(plan, p, M, 2 * H, epi, st, "gated_ffn");

@@ -263,6 +263,8 @@ static bool bad_dims(long M, long N, long K) {
   return M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00L || N > 0x7fffff00L || K > 131071;
 }
 
+inline Plan plan_of(long M, long N, long K) { return plan_tiles<int8_t>(M, N, stages<int8_t>(K), 1); }
+
 }  // namespace i8
 }  // namespace svk
 
@@ -305,6 +307,13 @@ extern "C" long svk_gemm_i8_workspace(const void* A, long lda, const void* W, lo
   return (tokens_ok(A, lda, K) ? 0 : M * ldk) + (rows_ok(W, ldw, K) ? 0 : N * ldk);
 }
 
+extern "C" int svk_gemm_i8_plan(long M, long N, long K, long* plan) {
+  if (bad_dims(M, N, K) || M == 0 || !plan) { set_error("svk_gemm_i8_plan: bad args"); return SVK_EINVAL; }
+  if (M <= SKINNY_M) tell_few(M, plan);
+  else tell(plan_of(M, N, K), M, plan);
+  return SVK_OK;
+}
+
 extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, const void* W, long ldw, const float* sw,
                            const float* bias, const void* R, long ldr, void* Y, long ldy, long M, long N, long K, int act,
                            void* ws, long ws_bytes, void* stream) {
@@ -345,7 +354,7 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
     p.nk = stages<int8_t>(p.K);
     p.abytes = (M - 1) * p.lda + p.K;
     p.bbytes = (N - 1) * p.ldb + p.K;
-    const Plan plan = plan_tiles<int8_t>(M, N, p.nk, 1);
+    const Plan plan = plan_of(M, N, K);
     auto run = [&](auto act_c) {
       ScaleEpi<T, decltype(act_c)::value> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0, past};
       return launch_plan<int8_t, false, false>(plan, p, M, N, epi, st, "gemm_i8");

@@ -391,6 +391,19 @@ inline Plan plan_tiles(long m, long n, long nk, long most) {
   return best;
 }
 
+// a plan as the host queries tell it: tile side, parts, rows, tile side of the rows behind them (0: none)
+inline void tell(const Plan& plan, long m, long* out) {
+  out[0] = 256 >> plan.tile;
+  out[1] = plan.parts;
+  out[2] = plan.rows;
+  out[3] = plan.rows < m ? 256 >> plan.rest : 0;
+}
+inline void tell_few(long m, long* out) {         // the few-token kernel has no tiles
+  out[0] = out[3] = 0;
+  out[1] = 1;
+  out[2] = m;
+}
+
 struct Slots { int cus, per; };
 template <class K>
 static Slots slots_of(K* fn, int threads) {

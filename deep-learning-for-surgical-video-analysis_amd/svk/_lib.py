@@ -120,6 +120,8 @@ SIGNATURES = {
     "svk_quant_rows": [c_int, P, c_long, P, c_long, P, c_long, c_long, P],
     "svk_gemm_i8": [c_int, P, c_long, P, P, c_long, P, P, P, c_long, P, c_long, c_long, c_long, c_long, c_int, P, c_long,
                     P],
+    "svk_gated_ffn_plan": [c_int, c_int, c_long, c_long, c_long, P],
+    "svk_gemm_i8_plan": [c_long, c_long, c_long, P],
 }
 STRING_FUNCS = ("svk_version", "svk_last_error", "svk_last_kernel")
 LONG_FUNCS = {"svk_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int, c_int],

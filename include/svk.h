@@ -623,6 +623,10 @@ long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void*
 int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH,
                       long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K, int act, void* ws,
                       long ws_bytes, void* stream);
+/* Host query: which tiles a product runs on.  product 0: the forward pass [M, 2H], 1: dX [M, K], 2: dW [2H, K].
+ * plan[4] = side of the square tiles (0: the few-token kernel), parts its reduction is split into, rows of the result that
+ * they cover, side of the tiles of the rows behind (0: none). */
+int svk_gated_ffn_plan(int dtype, int product, long M, long H, long K, long* plan);
 
 /* 8-bit integer products (csrc/gemm_i8.hip).  svk_quant_rows: S[m] = max |X[m, :]| * (1 / 127) in f32, Q[m, k] =
  * X[m, k] / S[m] rounded to the nearest integer (ties to even); a row of zeros has S = 0 and codes 0, a row with an infinity or a NaN S = NaN
@@ -633,6 +637,8 @@ int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ld
  * tokens, and where W's rows are whole aligned 16-byte pieces and A's are aligned and that far apart). */
 int svk_quant_rows(int dtype, const void* X, long ldx, void* Q, long ldq, float* S, long M, long K, void* stream);
 long svk_gemm_i8_workspace(const void* A, long lda, const void* W, long ldw, long M, long N, long K);
+/* Host query as svk_gated_ffn_plan, of Y [M, N]. */
+int svk_gemm_i8_plan(long M, long N, long K, long* plan);
 int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, const void* W, long ldw, const float* sw,
                 const float* bias, const void* R, long ldr, void* Y, long ldy, long M, long N, long K, int act, void* ws,
                 long ws_bytes, void* stream);

@@ -249,3 +249,21 @@ def test_rope3d_outputs_of_either_order_of_batch_and_time():
     for bad in ((40, 16, 1), (16, 40, 1), (31, 62, 1), (160, 31, 1), (100, 32, 1), (32, 40, 1), (0, 32, 1), (32, 0, 1), (200, 40, 2)):
         with pytest.raises(svk.SvkError, match="rows overlap"):
             ops._rope_out(q, None, (flat.as_strided((2, 5, 32), bad), None))
+
+
+def test_plan_queries():
+    import ctypes
+    from svk import ops
+    lib = _lib()
+    p = (ctypes.c_long * 4)()
+    for M in (1, ops._FEW):
+        assert lib.svk_gated_ffn_plan(1, 0, M, 32, 64, p) == 0 and list(p) == [0, 1, M, 0]
+        assert lib.svk_gemm_i8_plan(M, 32, 64, p) == 0 and list(p) == [0, 1, M, 0]
+    for dt in (0, 1, 2):
+        for product, rows in ((0, 16384), (1, 16384), (2, 11264)):
+            assert lib.svk_gated_ffn_plan(dt, product, 16384, 5632, 2048, p) == 0
+            assert p[0] in (64, 128, 256) and p[1] >= 1 and 0 < p[2] <= rows and (p[3] == 0) == (p[2] == rows) and p[3] < p[0]
+    assert lib.svk_gemm_i8_plan(16384, 8192, 4096, p) == 0 and list(p) == [256, 1, 16384, 0]
+    for bad in ((1, 3, 8, 8, 8), (1, -1, 8, 8, 8), (9, 0, 8, 8, 8), (1, 0, 0, 8, 8), (1, 0, 8, 0, 8), (1, 0, 8, 8, -1)):
+        assert lib.svk_gated_ffn_plan(*bad, p) == -1
+    assert lib.svk_gated_ffn_plan(1, 0, 8, 8, 8, None) == -1 and lib.svk_gemm_i8_plan(8, 8, 131072, p) == -1

@@ -665,6 +665,133 @@ def test_i8_refusals(cuda):
             ops.quant_rows(bad)
 
 
+# ---------------------------------------------------------------- every tile size, split and second launch
+
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _plan(entry, *args):
+    """(tile side, reduction split, tile side of the rows behind) that the library takes for these sizes."""
+    import ctypes
+    from svk import _lib
+    out = (ctypes.c_long * 4)()
+    _lib.call(entry, *args, out)
+    return out[0], out[1] > 1, out[3]
+
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+# tokens, hidden, K, (tile side, tile side of the last rows): H whole 16-byte pieces or odd
+_FWD16 = [(196, 4240, 152, (128, 0)), (16396, 35, 156, (128, 0)), (5124, 392, 848, (128, 64)), (2566, 787, 835, (128, 64)),
+          (24910, 208, 152, (256, 0)), (26051, 198, 154, (256, 0)), (22730, 332, 150, (256, 64)), (19628, 400, 322, (256, 128)),
+          (18545, 516, 258, (256, 128))]
+_FWD32 = [(24790, 40, 82, (128, 0)), (26594, 35, 76, (128, 0)), (33632, 162, 82, (128, 64)), (28379, 200, 80, (256, 0)),
+          (28213, 194, 75, (256, 0)), (34747, 196, 77, (256, 64)), (16426, 516, 77, (256, 128))]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dt,M,H,K,tiles", [(F32, *c) for c in _FWD32] + [(d, *c) for d in (BF16, F16) for c in _FWD16])
+def test_gated_ffn_every_tile(cuda, dt, M, H, K, tiles, act):
+    """With biases and kept projections; ReLU exact on integers, the others within test_gated_ffn_values' bounds."""
+    ops = _ops()
+    side, split, rest = _plan("svk_gated_ffn_plan", _CODE[dt], 0, M, H, K)
+    assert (side, rest) == tiles and not split
+    if act == "relu":
+        x, w, b = _ints(M, K, dt=dt, seed=1), _ints(2 * H, K, dt=dt, seed=2), _ints(2 * H, dt=F32, seed=3, top=3)
+        pre = x.to(F64) @ w.to(F64).t() + b.to(F64)
+        got, kept = ops.gated_ffn(x, w, b, act=act, save=True)
+        assert torch.equal(kept, pre.float().to(dt)) and torch.equal(got, (torch.relu(pre[:, :H]) * pre[:, H:]).float().to(dt))
+        return
+    x, w = _rand(M, K, dt=dt, seed=1, scale=2.0), _rand(2 * H, K, dt=dt, seed=2, scale=K ** -0.5)
+    b = _rand(2 * H, dt=F32, seed=3)
+    X, W = x.to(F64), w.to(F64)
+    pre = X @ W.t() + b.to(F64)
+    e = (K + 2) * 2.0 ** -24 * (X.abs() @ W.abs().t() + b.to(F64).abs())
+    g, u, eg, eu = pre[:, :H], pre[:, H:], e[:, :H], e[:, H:]
+    ref = _act64(g, act) * u
+    tol = 1.2 * eg * (u.abs() + eu) + _act64(g, act).abs() * eu + g.abs() * u.abs() * 2.0 ** -21
+    got, kept = ops.gated_ffn(x, w, b, act=act, save=True)
+    _within(got, ref, U[dt] * (ref.abs() + tol) + tol + 2.0 ** -25, "h")
+    _within(kept, pre, U[dt] * (pre.abs() + e) + e + 2.0 ** -25, "pre")
+
+
+# product (1: dx, 2: dW), tokens, hidden, K, (tile side, split, tile side of the last rows)
+_BWD16 = [(1, 10982, 80, 136, (128, False, 0)), (1, 3301, 420, 1235, (128, False, 64)), (1, 513, 4531, 67, (128, True, 0)),
+          (1, 24757, 80, 408, (256, False, 0)), (1, 16698, 75, 652, (256, False, 0)), (1, 33473, 82, 385, (256, False, 64)),
+          (1, 33155, 130, 544, (256, False, 128)), (1, 4370, 2674, 195, (256, True, 0)), (2, 155, 4208, 200, (128, False, 0)),
+          (2, 833, 2505, 803, (128, False, 64)), (2, 4874, 33, 1043, (128, True, 0)), (2, 156, 4108, 1415, (256, False, 0)),
+          (2, 164, 4676, 1674, (256, False, 64)), (2, 325, 4734, 1797, (256, False, 128)), (2, 5378, 2056, 200, (256, True, 0))]
+_BWD32 = [(1, 26259, 38, 66, (128, False, 0)), (1, 33398, 39, 327, (128, False, 64)), (1, 4133, 517, 66, (128, True, 0)),
+          (1, 6344, 41, 1930, (256, False, 0)), (1, 21829, 39, 663, (256, False, 64)), (1, 26475, 40, 642, (256, False, 128)),
+          (1, 1489, 1096, 656, (256, True, 0)), (2, 78, 5062, 266, (128, False, 0)), (2, 129, 3910, 1153, (128, False, 64)),
+          (2, 1029, 371, 641, (128, True, 0)), (2, 80, 5515, 1102, (256, False, 0)), (2, 79, 4785, 1667, (256, False, 64)),
+          (2, 77, 5728, 1544, (256, False, 128)), (2, 4413, 1040, 216, (256, True, 0))]
+
+
+@pytest.mark.parametrize("dt,product,M,H,K,plan", [(F32, *c) for c in _BWD32] + [(d, *c) for d in (BF16, F16) for c in _BWD16])
+def test_gated_ffn_bwd_every_tile(cuda, dt, product, M, H, K, plan):
+    """Integers as in test_gated_ffn_bwd_exact; the sums stay under 4 * 34000 < 2^24."""
+    ops = _ops()
+    assert _plan("svk_gated_ffn_plan", _CODE[dt], product, M, H, K) == plan
+    x, w = _ints(M, K, dt=dt, seed=4), _ints(2 * H, K, dt=dt, seed=5)
+    pre, dh = _ints(M, 2 * H, dt=dt, seed=6, top=2), _ints(M, H, dt=dt, seed=7, top=2)
+    g, u, d = pre[:, :H].to(F64), pre[:, H:].to(F64), dh.to(F64)
+    dp = torch.cat([d * u * (g > 0), d * torch.relu(g)], 1)
+    dx, dw, db = ops.gated_ffn_bwd(x, w, pre, dh, act="relu")
+    assert torch.equal(dx, (dp @ w.to(F64)).float().to(dt))
+    assert torch.equal(dw, (dp.t().contiguous() @ x.to(F64)).float().to(dt))
+    assert torch.equal(db, dp.sum(0).float())
+
+
+_I8 = [(16416, 74, 315, (128, 0)), (17310, 72, 300, (128, 0)), (33444, 72, 1145, (128, 64)), (25289, 400, 332, (256, 0)),
+       (25127, 434, 303, (256, 0)), (33836, 388, 309, (256, 64)), (15836, 2128, 307, (256, 128))]
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("M,N,K,tiles", _I8)
+def test_gemm_i8_every_tile(cuda, dt, M, N, K, tiles):
+    """Scales, bias, every activation and a residual that is also the output, within test_gemm_i8's bounds."""
+    ops = _ops()
+    side, split, rest = _plan("svk_gemm_i8_plan", M, N, K)
+    assert (side, rest) == tiles and not split
+    a, w = _codes(M, K, 1), _codes(N, K, 2)
+    sa, sw = _rand(M, dt=F32, seed=3).abs() / 64, _rand(N, dt=F32, seed=4).abs() / 64
+    b, r = _rand(N, dt=F32, seed=5), _rand(M, N, dt=dt, seed=6)
+    y = (a.to(F64) @ w.to(F64).t()) * sa.to(F64)[:, None] * sw.to(F64)
+    for act, bias, res in ((None, None, None), ("gelu", b, r), ("relu", b, r), ("tanh", b, None), (None, b, r)):
+        z = y if bias is None else y + bias.to(F64)
+        v = {None: z, "gelu": z * torch.special.ndtr(z), "relu": torch.relu(z), "tanh": torch.tanh(z)}[act]
+        ref = v if res is None else v + res.to(F64)
+        tol = 1.2 * 4 * 2.0 ** -24 * (y.abs() + (0 if bias is None else bias.to(F64).abs())) + z.abs() * 2.0 ** -21
+        tol = tol + 2.0 ** -24 * (ref.abs() + v.abs())
+        got = ops.gemm_i8(a, sa, w, sw, bias, act=act, residual=res, dtype=dt)
+        _within(got, ref, U[dt] * (ref.abs() + tol) + tol + 2.0 ** -25, f"{act}")
+        if res is not None:
+            own = res.clone()
+            ops.gemm_i8(a, sa, w, sw, bias, act=act, residual=own, out=own)
+            assert torch.equal(own, got)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("width", [1500, 3001, 5000, 7003])
+@pytest.mark.parametrize("K", [77, 2304])
+def test_few_tokens_every_width(cuda, dt, width, K):
+    """One to four blocks of weight rows a workgroup, one to four blocks of tokens, rows that end inside a piece and rows
+    of several turns of the waves; all exact."""
+    ops = _ops()
+    w, b = _ints(2 * width, K, dt=dt, seed=2), _ints(2 * width, dt=F32, seed=3, top=3)
+    wq, one = _codes(2 * width, K, 4), torch.ones(2 * width, device="cuda")
+    for M in (1, 16, 20, 33, 64):
+        x = _ints(M, K, dt=dt, seed=M)
+        pre = x.to(F64) @ w.to(F64).t() + b.to(F64)
+        ref = torch.relu(pre[:, :width]) * pre[:, width:]
+        assert float(ref.abs().max()) < 2 ** 24
+        h, kept = ops.gated_ffn(x, w, b, act="relu", save=True)
+        assert torch.equal(h, ref.float().to(dt)) and torch.equal(kept, pre.float().to(dt))
+        a = _codes(M, K, M)
+        want = (a.to(F64) @ wq.to(F64).t()).float()
+        assert torch.equal(ops.gemm_i8(a, one[:M], wq, one, dtype=F32), want)
+
+
 # ---------------------------------------------------------------- together
 
 def _block(ops, x, pos, freqs, p, eps=1e-6):
