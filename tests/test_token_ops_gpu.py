@@ -665,6 +665,32 @@ def test_i8_refusals(cuda):
             ops.quant_rows(bad)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [40, 4000])
+def test_gelu_of_16_bit_results_down_its_tail(cuda, dt, M):
+    """GELU(g) alone (up = 1), as gated_ffn and gemm_i8 form it.  erfc is off by 1.5e-7 at most, so the result by
+    0.75e-7 |g|, and six f32 roundings of a correction of at most |g| / 2; as the correction is a positive multiple of
+    exp(-g^2 / 2) that tends to 0.7779 / 0.5642 of the true one, the tail is within 0.4 of itself as well.  Then half a
+    step (f16: half the smallest one, 2^-25)."""
+    ops = _ops()
+    g = torch.linspace(-12, 9, M).to(dt).cuda()
+    x, w = torch.ones(M, 8, device="cuda", dtype=dt), torch.zeros(32, 8, device="cuda", dtype=dt)
+    x[:, 0] = g
+    w[:16, 0] = w[16:, 1] = 1
+    h = ops.gated_ffn(x, w, act="gelu")
+    G = g.to(F64)
+    ref = G * 0.5 * torch.erfc(-G * 0.5 ** 0.5)        # (ndtr cancels in 64 bits: 0 from -8.3 down)
+    err = 0.75e-7 * G.abs() + 6 * 2.0 ** -24 * G.abs() / 2 + 2.0 ** -24 * ref.abs()
+    err = torch.where(G < -2, torch.minimum(err, 0.4 * ref.abs()), err)
+    tol = err + U[dt] * (ref.abs() + err) + (2.0 ** -25 if dt == torch.float16 else 2.0 ** -134)
+    _within(h, ref[:, None].expand(M, 16), tol[:, None].expand(M, 16), "gated")
+    # 8-bit: codes times scales that give the same arguments (one product of powers of two, so exact)
+    a = torch.ones(M, 16, device="cuda", dtype=torch.int8)
+    one = torch.ones(16, 16, device="cuda", dtype=torch.int8)
+    y = ops.gemm_i8(a, g.float() / 16, one, torch.ones(16, device="cuda"), act="gelu", dtype=dt)
+    _within(y, ref[:, None].expand(M, 16), tol[:, None].expand(M, 16), "i8")
+
+
 # ---------------------------------------------------------------- every tile size, split and second launch
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
