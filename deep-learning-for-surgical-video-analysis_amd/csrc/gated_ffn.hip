@@ -63,7 +63,7 @@ struct GateEpi {
   T* pre;                 // [M, 2H] contiguous, or null
   const float* bias;      // [2H] or null
   int M, H, act, per;
-  bool past;              // rows of h and pre are whole 16-byte pieces
+  bool past;              // rows of h and pre are whole lines
   void skip(long rows) {
     h += rows * ldh;
     if (pre) pre += rows * 2 * H;
@@ -144,7 +144,7 @@ struct PlainEpi {
   T* y; long ldy;
   float* slab;            // [parts][M][N], or null
   int M, N;
-  bool past;              // rows of y are whole 16-byte pieces
+  bool past;              // rows of y are whole lines
   void skip(long rows) { y += rows * ldy; }      // never with slabs
   template <class C, typename A>
   __device__ __forceinline__ void write(A (&acc)[C::TM][C::TN], int m0, int tn, int wn, int fq, int part) const {
@@ -382,7 +382,7 @@ extern "C" int svk_gated_ffn(int dtype, const void* X, long ldx, const void* W, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
-    const bool past = al16(Hout) && ldh * es % 16 == 0 && H * es % 16 == 0 && al16(pre);
+    const bool past = whole_lines(Hout, ldh * es, H * es) && (!pre || whole_lines(pre, 0, 0));
     Args p{(const char*)X, (const char*)W, ldx * es, ldw * es, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       GateEpi<T, -1> epi{(T*)Hout, ldh, (T*)pre, bias, (int)M, (int)H, act, 0, past};
@@ -485,7 +485,7 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, Slabs& j, const char* name) -> int {
       p.nk = stages<T>(p.K);
       float* slabs = plan.parts > 1 ? (float*)at : nullptr;
-      PlainEpi<T> epi{y, ldy, slabs, (int)m, (int)n, al16(y) && ldy * es % 16 == 0 && n * es % 16 == 0};
+      PlainEpi<T> epi{y, ldy, slabs, (int)m, (int)n, whole_lines(y, ldy * es, n * es)};
       if (slabs) {
         j = Slabs{slabs, y, ldy, plan.parts, (int)m, (int)n, blocks_of(m * n)};
         at += up16(plan.parts * m * n * 4);

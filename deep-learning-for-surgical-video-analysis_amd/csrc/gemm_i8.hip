@@ -165,7 +165,7 @@ struct ScaleEpi {
   const T* R; long ldr;
   T* y; long ldy;
   int M, N, act, per;
-  bool past;              // rows of y are whole 16-byte pieces
+  bool past;              // rows of y are whole lines
   void skip(long rows) {
     sa += rows;
     if (R) R += rows * ldr;
@@ -332,7 +332,7 @@ extern "C" int svk_gemm_i8(int dtype, const void* A, long lda, const float* sa, 
   if (M == 0) return SVK_OK;
   hipStream_t st = (hipStream_t)stream;
   SVK_DISPATCH_DTYPE(dtype, T, {
-    const bool past = al16(Y) && ldy * (long)sizeof(T) % 16 == 0 && N * (long)sizeof(T) % 16 == 0;
+    const bool past = whole_lines(Y, ldy * (long)sizeof(T), N * (long)sizeof(T));
     Args p{(const char*)A, (const char*)W, lda, ldw, 0, 0, (int)M, (int)K, 0, 0, 0, 1};
     if (M <= SKINNY_M) {
       ScaleEpi<T, -1> epi{sa, sw, bias, (const T*)R, ldr, (T*)Y, ldy, (int)M, (int)N, act, 0, past};

@@ -115,8 +115,7 @@ __device__ __forceinline__ void tile_of(int bid, int ntm, int ntn, int& tm, int&
   tn = in / g;
 }
 
-// W consecutive values of a row: one store (of any alignment) where all W exist, else one by one.  NTS: past the L2;
-// only for rows of whole 16-byte pieces (partial lines past the L2 cost: 50176 x 320 x 2 x 853 in f16 107 us, 99 without)
+// W consecutive values of a row: one store (of any alignment) where all W exist, else one by one.  NTS: past the L2
 template <typename T, int W, bool NTS>
 __device__ __forceinline__ void put(T* at, const float* v, int n) {
   T o[W];
@@ -591,6 +590,13 @@ static int pad(const void* X, long ldx, void* Y, long rows, long kbytes, hipStre
   return check_launch("pad_rows");
 }
 
+// rows that may be stored past the L2: whole 64-byte lines.  Lines that two tiles share cost there what they would not in the
+// L2 (8-bit products of 50176 x 320 with 680 results in f16, rows of 21.25 lines: 77 us, 43 through the L2; 16384 x 1024 with
+// 1000: 47 and 31; 50176 x 320 x 2 x 856 in bf16: 93 and 87); whole lines gain by it (16384 x 4096 with 8192: 446 us, 473
+// through the L2; with 8224: 491 and 539).  Long reductions are within 3 % either way
+inline bool whole_lines(const void* p, long ld_bytes, long row_bytes) {
+  return (((uintptr_t)p | (uintptr_t)ld_bytes | (uintptr_t)row_bytes) & 63) == 0;
+}
 inline long up16(long bytes) { return (bytes + 15) & ~15L; }
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

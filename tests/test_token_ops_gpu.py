@@ -706,11 +706,11 @@ def _plan(entry, *args):
 
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
-# tokens, hidden, K, (tile side, tile side of the last rows): H whole 16-byte pieces or odd
+# tokens, hidden, K, (tile side, tile side of the last rows); rows of results of whole 64-byte lines and of any length
 _FWD16 = [(196, 4240, 152, (128, 0)), (16396, 35, 156, (128, 0)), (5124, 392, 848, (128, 64)), (2566, 787, 835, (128, 64)),
-          (24910, 208, 152, (256, 0)), (26051, 198, 154, (256, 0)), (22730, 332, 150, (256, 64)), (19628, 400, 322, (256, 128)),
+          (24910, 208, 152, (256, 0)), (24910, 224, 152, (256, 0)), (26051, 198, 154, (256, 0)), (22730, 332, 150, (256, 64)), (19628, 400, 322, (256, 128)),
           (18545, 516, 258, (256, 128))]
-_FWD32 = [(24790, 40, 82, (128, 0)), (26594, 35, 76, (128, 0)), (33632, 162, 82, (128, 64)), (28379, 200, 80, (256, 0)),
+_FWD32 = [(24790, 40, 82, (128, 0)), (26594, 35, 76, (128, 0)), (33632, 162, 82, (128, 64)), (28379, 200, 80, (256, 0)), (28379, 208, 80, (256, 0)),
           (28213, 194, 75, (256, 0)), (34747, 196, 77, (256, 64)), (16426, 516, 77, (256, 128))]
 
 
@@ -742,14 +742,14 @@ def test_gated_ffn_every_tile(cuda, dt, M, H, K, tiles, act):
 
 # product (1: dx, 2: dW), tokens, hidden, K, (tile side, split, tile side of the last rows)
 _BWD16 = [(1, 10982, 80, 136, (128, False, 0)), (1, 3301, 420, 1235, (128, False, 64)), (1, 513, 4531, 67, (128, True, 0)),
-          (1, 24757, 80, 408, (256, False, 0)), (1, 16698, 75, 652, (256, False, 0)), (1, 33473, 82, 385, (256, False, 64)),
+          (1, 24757, 80, 408, (256, False, 0)), (1, 24757, 80, 416, (256, False, 0)), (1, 16698, 75, 652, (256, False, 0)), (1, 33473, 82, 385, (256, False, 64)),
           (1, 33155, 130, 544, (256, False, 128)), (1, 4370, 2674, 195, (256, True, 0)), (2, 155, 4208, 200, (128, False, 0)),
           (2, 833, 2505, 803, (128, False, 64)), (2, 4874, 33, 1043, (128, True, 0)), (2, 156, 4108, 1415, (256, False, 0)),
-          (2, 164, 4676, 1674, (256, False, 64)), (2, 325, 4734, 1797, (256, False, 128)), (2, 5378, 2056, 200, (256, True, 0))]
+          (2, 164, 4676, 1674, (256, False, 64)), (2, 325, 4734, 1797, (256, False, 128)), (2, 325, 4734, 1792, (256, False, 64)), (2, 5378, 2056, 200, (256, True, 0))]
 _BWD32 = [(1, 26259, 38, 66, (128, False, 0)), (1, 33398, 39, 327, (128, False, 64)), (1, 4133, 517, 66, (128, True, 0)),
-          (1, 6344, 41, 1930, (256, False, 0)), (1, 21829, 39, 663, (256, False, 64)), (1, 26475, 40, 642, (256, False, 128)),
+          (1, 6344, 41, 1930, (256, False, 0)), (1, 15190, 40, 784, (256, False, 0)), (1, 21829, 39, 663, (256, False, 64)), (1, 26475, 40, 642, (256, False, 128)),
           (1, 1489, 1096, 656, (256, True, 0)), (2, 78, 5062, 266, (128, False, 0)), (2, 129, 3910, 1153, (128, False, 64)),
-          (2, 1029, 371, 641, (128, True, 0)), (2, 80, 5515, 1102, (256, False, 0)), (2, 79, 4785, 1667, (256, False, 64)),
+          (2, 1029, 371, 641, (128, True, 0)), (2, 80, 5515, 1102, (256, False, 0)), (2, 80, 5515, 1104, (256, False, 0)), (2, 79, 4785, 1667, (256, False, 64)),
           (2, 77, 5728, 1544, (256, False, 128)), (2, 4413, 1040, 216, (256, True, 0))]
 
 
@@ -768,7 +768,7 @@ def test_gated_ffn_bwd_every_tile(cuda, dt, product, M, H, K, plan):
     assert torch.equal(db, dp.sum(0).float())
 
 
-_I8 = [(16416, 74, 315, (128, 0)), (17310, 72, 300, (128, 0)), (33444, 72, 1145, (128, 64)), (25289, 400, 332, (256, 0)),
+_I8 = [(16416, 74, 315, (128, 0)), (17310, 72, 300, (128, 0)), (33444, 72, 1145, (128, 64)), (25289, 400, 332, (256, 0)), (25289, 416, 332, (256, 0)),
        (25127, 434, 303, (256, 0)), (33836, 388, 309, (256, 64)), (15836, 2128, 307, (256, 128))]
 
 
