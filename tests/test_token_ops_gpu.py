@@ -494,6 +494,20 @@ def test_quant_rows_has_the_codes_of_the_torch_expression(cuda, dt):
     assert torch.equal(sc, s) and torch.equal(q.float(), torch.round(x.float() / s[:, None]))
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("K", [17, 333, 512, 1000])
+def test_quant_rows_of_many_short_rows(cuda, dt, K):
+    """One row a wave or several: the same bits."""
+    ops = _ops()
+    x = _rand(7003, K, dt=dt, seed=3)
+    q, s = ops.quant_rows(x)
+    xf = x.float().cpu()
+    want = xf.abs().amax(1) * _127TH
+    assert torch.equal(s.cpu(), want) and torch.equal(q.cpu(), torch.round(xf / want[:, None]).to(torch.int8))
+    few = ops.quant_rows(x[-600:])
+    assert torch.equal(q[-600:], few[0]) and torch.equal(s[-600:], few[1])
+
+
 def test_quant_rows_more_rows_than_one_launch(cuda):
     """2^26 rows, 64 threads each, are 2^32 threads."""
     ops = _ops()
