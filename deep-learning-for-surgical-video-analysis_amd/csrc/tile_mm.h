@@ -347,9 +347,12 @@ using Small = Tile<64, 64, 2, 2, 3, 3>;        // three
 
 // Which tile, and into how many parts the reduction is split where `most` allows it (parts are f32 slabs that another
 // kernel joins).  A CU works off its tiles at `step` us a stage with its residents together, but no stage of one tile in
-// less than `alone` us; `end` us a tile for its results.  Measured on 1 to 50176 rows, 96 to 5632 results, 64 to 2048
-// values of k; the choice is the best of the three, or within 10 % of it, at nearly all of them (1500 x 1024 x 2 x 5632
-// in bf16: 128-wide 50, 256-wide 57, 64-wide 68 us; 6000 x 2048 x 2 x 1024: 60, 51, 95; 100 x 2048 x 2 x 340: 24, 45, 14).
+// less than `alone` us; `end` us a tile for its results.  Fitted over 100 to 50176 rows, 192 to 11264 results, 64 to 2048
+// values of k (profiles/token_ops/choices.txt): the choice is the best of the three tiles or within 10 % of it at 359 of
+// 388 sizes, within 20 % at 381 (bf16, 256-, 128-, 64-wide: 1500 x 1024 x 2 x 5632 55, 51, 66 us, chosen 48; 6000 x 2048 x
+// 2 x 1024 52, 61, 90, chosen 60; 100 x 2048 x 2 x 340 45, 28, 14, chosen 14).  `end` is one number a type: it does not know
+// the activation, kept projections, a residual or rows that are no whole lines, and it is there that the choice is wrong
+// by more (8 bits, 50176 x 64 with 680 results in f16: 45 us, 128-wide 27).
 // Where the last round of tiles would leave most CUs idle, the rows behind the whole rounds are taken by a second launch
 // with smaller tiles (352 tiles of 256 for 256 CUs, dW of 8192 tokens: 421 -> 388 us).
 struct Plan { int tile, parts; long rows; int rest; };          // the first `rows` rows with `tile`, the others with `rest`
@@ -458,6 +461,9 @@ template <typename T> inline int stages(long k) { return (int)((k * (long)sizeof
 // split over the workgroup's waves and joined in LDS.  MT blocks of 16 tokens, NB blocks of 16 weight rows a workgroup
 // (the epilogue's map names them, `epi.per` results).  Rows of any alignment and length.  Bound by the weights' bytes, and below some MiB by one trip to memory.
 constexpr int SK_WAVES = 8;
+// up to which it runs (us of it | of the tiles, weights of several copies in turn from memory: 2048 -> 2 x 5632 in bf16 1 token
+// 13.4 | 17.5, 32 17.6 | 18.1, 48 20.8 | 18.2, 64 21.8 | 18.9; 2048 -> 2 x 340 64 tokens 11.9 | 14.1; 512 -> 2 x 2048 in f32
+// 8.8 | 14.9; 8 bits 4096 -> 8192 18.2 | 17.4, 2048 -> 2048 7.5 | 8.7: at 64 tokens ahead but for the widest weights)
 constexpr int SKINNY_M = 64;
 
 // 16 bytes of a row from byte kb on, zeros past its end; rows of any alignment (the hardware reads 16 bytes anywhere)

@@ -1553,16 +1553,27 @@ def _vector(t, n, dev, fn, name):
         raise _lib.SvkError(f"svk.{fn}: {name} must be {n} contiguous float32 values, got {tuple(t.shape)}")
 
 
+def _span(t):
+    """(first, one behind the last) byte of a tensor's elements."""
+    p = t.data_ptr()
+    if t.numel() == 0:
+        return p, p
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _apart(a, b, same=True):
     """False where writing ``a`` may change ``b``: their memory meets, and they are neither two column ranges of one
     buffer's rows nor (``same``: where every value of b is read by who writes it) the same elements in the same order."""
-    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
+    if a is None or b is None:
         return True
-    ea, eb = a.element_size(), b.element_size()
-    last = lambda t, e: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * e  # noqa: E731
-    if last(a, ea) <= b.data_ptr() or last(b, eb) <= a.data_ptr():
-        return True
-    if ea != eb:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1 or _interleaved(a, b, same)
+
+
+def _interleaved(a, b, same):
+    """_apart of two tensors whose spans meet."""
+    ea = a.element_size()
+    if ea != b.element_size():
         return False
     if a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride():
         return same
@@ -1592,21 +1603,30 @@ def _rope_out(q, k, out, *tables):
     qo, ko = out
     if (ko is None) != (k is None):
         raise _lib.SvkError("svk.rope3d: out must be (q', k') like (q, k)")
+    spans = []
     for o, t, nm in ((qo, q, "q"), (ko, k, "k")):
         if t is None:
             continue
-        _like(o, q.dtype, q.get_device(), "rope3d", "out")
-        if o.shape != t.shape:
-            raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
-        width, run = t.shape[2], t.shape[2]
-        good = width == 1 or o.stride(2) == 1
-        for s, n in sorted((o.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1):       # either may be the outer dim
-            good, run = good and s >= run, s * (n - 1) + width
-        if not good:
+        if o is not t:
+            _like(o, q.dtype, q.get_device(), "rope3d", "out")
+            if o.shape != t.shape:
+                raise _lib.SvkError(f"svk.rope3d: out for {nm} is {tuple(o.shape)}, not {tuple(t.shape)}")
+        (B, N, width), (sb, sn, sc) = t.shape, o.stride()
+        if (width > 1 and sc != 1) or (N > 1 and sn < width) or (B > 1 and sb < width) or \
+                (B > 1 and N > 1 and sb < sn * (N - 1) + width and sn < sb * (B - 1) + width):     # either may be outside
             raise _lib.SvkError("svk.rope3d: out rows overlap or lack unit channel stride")
-    if not (_apart(qo, q) and _apart(ko, k) and _apart(qo, k, same=False) and _apart(ko, q, same=False) and
-            _apart(qo, ko, same=False) and all(_apart(o, t, same=False) for o in (qo, ko) for t in tables)):
-        raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
+        p = o.data_ptr()
+        spans.append((p, p + ((B - 1) * sb + (N - 1) * sn + width) * o.element_size() if B and N else p, o))
+    meet = [(spans[0], _s, False) for _s in spans[1:]]
+    for i, (o, own, cross) in enumerate(((qo, q, k), (ko, k, q))[:len(spans)]):
+        if o is not own:
+            meet.append((spans[i], (*_span(own), own), True))
+        if cross is not None and not (qo is q and ko is k):          # in place the other input is the other output
+            meet.append((spans[i], (*_span(cross), cross), False))
+        meet += [(spans[i], (*_span(t), t), False) for t in tables]
+    for (a0, a1, a), (b0, b1, b), same in meet:
+        if max(a0, b0) < min(a1, b1) and not _interleaved(a, b, same):
+            raise _lib.SvkError("svk.rope3d: out overlaps the inputs or itself")
     return qo, ko
 
 
