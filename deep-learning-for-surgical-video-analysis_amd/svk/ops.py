@@ -1736,7 +1736,9 @@ def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
 
 def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
     """Gradients (dx, dw, db) of gated_ffn from dh [..., hidden] and the saved ``pre``: dx like x, dw [2 * hidden, K] in
-    w's dtype, db float32 [2 * hidden]; None where not asked for.  Written, not added to; the same bits on every run."""
+    w's dtype, db float32 [2 * hidden]; None where not asked for.  Written, not added to; the same bits on every run.
+    The gradients of the projections are rounded once to x's dtype before the two products (db sums them unrounded);
+    float32 operands keep them in 32 bits."""
     fn = "gated_ffn_bwd"
     dt, dev, M, K, ldx, ldw, H = _gated_args(x, w, fn)
     code = _glu(act, fn)
