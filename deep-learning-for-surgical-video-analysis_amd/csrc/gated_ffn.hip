@@ -138,10 +138,25 @@ struct GateEpi {
   }
 };
 
-// plain product of a col operand B: rounded to T, or an f32 slab of one part of the reduction
-template <typename T>
+// v += the first n (of 4) values at `at`
+__device__ __forceinline__ void add_to(float* v, const float* at, int n) {
+  typedef f32x4 anywhere __attribute__((aligned(4)));
+  if (n >= 4) {
+    const f32x4 o = *reinterpret_cast<const anywhere*>(at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += o[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) v[e] += at[e];
+  }
+}
+
+// plain product of a col operand B: rounded to T; or (ADD) added in f32 to y; or an f32 slab of one part of the reduction
+template <typename T, bool ADD>
 struct PlainEpi {
-  T* y; long ldy;
+  typedef std::conditional_t<ADD, float, T> out_t;
+  out_t* y; long ldy;
   float* slab;            // [parts][M][N], or null
   int M, N;
   bool past;              // rows of y are whole lines
@@ -161,9 +176,14 @@ struct PlainEpi {
       for (int i = 0; i < C::TM; ++i) {
         const int m = m0 + i * 16;
         if (m >= M) continue;
-        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (slab) put<float, 4, false>(slab + ((long)part * M + m) * N + n, v, left);
-        else put<T, 4, NTS>(y + (long)m * ldy + n, v, left);
+        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (slab) {
+          put<float, 4, false>(slab + ((long)part * M + m) * N + n, v, left);
+          continue;
+        }
+        out_t* at = y + (long)m * ldy + n;
+        if constexpr (ADD) add_to(v, at, left);
+        put<out_t, 4, NTS>(at, v, left);
       }
     }
   }
@@ -175,9 +195,10 @@ struct Slabs {
   const float* S;         // [parts][M][N]
   void* y; long ldy;
   int parts, M, N, blocks;        // workgroups that join it
+  bool add;               // y is f32 and added to
 };
 constexpr int JOIN = 4;   // values a thread
-template <typename T>
+template <typename T, bool ADD>
 __device__ __forceinline__ void join_slabs(const Slabs& j, int block) {
   const long total = (long)j.M * j.N;
   T* y = static_cast<T*>(j.y);
@@ -197,20 +218,27 @@ __device__ __forceinline__ void join_slabs(const Slabs& j, int block) {
     }
     const long m = i / j.N;
     const int n = (int)(i - m * j.N);
-    if (n + JOIN <= j.N) put<T, JOIN, false>(y + m * j.ldy + n, v, JOIN);
-    else
+    if (n + JOIN <= j.N) {
+      if constexpr (ADD) add_to(v, y + m * j.ldy + n, JOIN);
+      put<T, JOIN, false>(y + m * j.ldy + n, v, JOIN);
+    } else {
 #pragma unroll
       for (int e = 0; e < JOIN; ++e)
-        if (i + e < total) y[(i + e) / j.N * j.ldy + (i + e) % j.N] = from_f<T>(v[e]);
+        if (i + e < total) {
+          T* at = y + (i + e) / j.N * j.ldy + (i + e) % j.N;
+          if constexpr (ADD) v[e] += *at;
+          *at = from_f<T>(v[e]);
+        }
+    }
   }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void join_all(Slabs x, Slabs w, const float* __restrict__ S, int rows, float* __restrict__ db,
-                                                int N) {
+                                                int N, bool add) {
   int b = blockIdx.x;
-  if (b < x.blocks) return join_slabs<T>(x, b);
+  if (b < x.blocks) return join_slabs<T, false>(x, b);
   b -= x.blocks;
-  if (b < w.blocks) return join_slabs<T>(w, b);
+  if (b < w.blocks) return w.add ? join_slabs<float, true>(w, b) : join_slabs<T, false>(w, b);
   b -= w.blocks;
   // 16 columns a workgroup, 16 threads a column
   __shared__ float part[16][17];
@@ -224,7 +252,7 @@ __global__ __launch_bounds__(256) void join_all(Slabs x, Slabs w, const float* _
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += part[i][cl];
-    db[c] = s;
+    db[c] = add ? db[c] + s : s;
   }
 }
 
@@ -440,9 +468,10 @@ extern "C" long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, 
   return BwdWs(es, M, H, K, padx, want_db, want_dx, want_dw).total;
 }
 
-extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre,
-                                 const void* dH, long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K,
-                                 int act, void* ws, long ws_bytes, void* stream) {
+// add: SVK_ADD_DW (dW is f32), SVK_ADD_DB
+static int backward(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH, long lddh,
+                    void* dX, long lddx, void* dW, float* db, int add, long M, long H, long K, int act, void* ws, long ws_bytes,
+                    void* stream) {
   const long es = es_of(dtype);
   if (!es) { set_error("svk_gated_ffn_bwd: unsupported dtype %d", dtype); return SVK_EINVAL; }
   if (!X || !W || !pre || !dH || bad_dims(M, H, K) || ldx < K || ldw < K || lddh < H || (dX && lddx < K) ||
@@ -459,6 +488,7 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
   const BwdWs need(es, M, H, K, padx, db, dX, dW);
   if (M && (!ws || !al16(ws) || ws_bytes < need.total)) { set_error("svk_gated_ffn_bwd: workspace too small or misaligned"); return SVK_EINVAL; }
   hipStream_t st = (hipStream_t)stream;
+  const bool add_w = add & SVK_ADD_DW, add_b = add & SVK_ADD_DB;
   SVK_DISPATCH_DTYPE(dtype, T, {
     auto blocks_of = [](long values) { return (int)std::min<long>((values + 256 * JOIN - 1) / (256 * JOIN), 4096); };
     Slabs jx{};
@@ -467,11 +497,11 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     auto join = [&](const float* sums, int rows) -> int {
       const int all = jx.blocks + jw.blocks + db_blocks;
       if (!all) return SVK_OK;
-      hipLaunchKernelGGL((join_all<T>), dim3((unsigned)all), dim3(256), 0, st, jx, jw, sums, rows, db, (int)(2 * H));
+      hipLaunchKernelGGL((join_all<T>), dim3((unsigned)all), dim3(256), 0, st, jx, jw, sums, rows, db, (int)(2 * H), add_b);
       return check_launch("join_all");
     };
     if (M == 0) {                                   // no tokens: the sums are empty
-      if (dW) jw = Slabs{nullptr, dW, K, 0, (int)(2 * H), (int)K, blocks_of(2 * H * K)};
+      if (dW && !add_w) jw = Slabs{nullptr, dW, K, 0, (int)(2 * H), (int)K, blocks_of(2 * H * K), false};
       return join(nullptr, 0);
     }
     char* at = (char*)ws;
@@ -498,12 +528,14 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
                        (const T*)pre, (const T*)dH, lddh, D, need.ldd, sums, (int)M, (int)H, act, need.rows);
     if (int rc = check_launch("gated_dpre")) return rc;
     // y [m, n]; where its reduction is split, the parts' slabs, joined below
-    auto product = [&](auto ac, Plan plan, Args p, T* y, long ldy, long m, long n, Slabs& j, const char* name) -> int {
+    auto product = [&](auto ac, auto addc, Plan plan, Args p, void* y, long ldy, long m, long n, Slabs& j, const char* name) -> int {
+      typedef PlainEpi<T, decltype(addc)::value> Epi;
+      constexpr long out = sizeof(typename Epi::out_t);
       p.nk = stages<T>(p.K);
       float* slabs = plan.parts > 1 ? (float*)at : nullptr;
-      PlainEpi<T> epi{y, ldy, slabs, (int)m, (int)n, whole_lines(y, ldy * es, n * es)};
+      Epi epi{(typename Epi::out_t*)y, ldy, slabs, (int)m, (int)n, whole_lines(y, ldy * out, n * out)};
       if (slabs) {
-        j = Slabs{slabs, y, ldy, plan.parts, (int)m, (int)n, blocks_of(m * n)};
+        j = Slabs{slabs, y, ldy, plan.parts, (int)m, (int)n, blocks_of(m * n), decltype(addc)::value};
         at += up16(plan.parts * m * n * 4);
       }
       return launch_plan<T, decltype(ac)::value, true>(plan, p, m, n, epi, st, name);
@@ -511,9 +543,27 @@ extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void*
     const long Db = M * need.ldd * es;
     // the padding of D is zero and rows of W past 2H read as zero, so dx's reduction runs over whole chunks
     if (dX)
-      if (int rc = product(std::false_type{}, need.px, Args{(const char*)D, Wr, need.ldd * es, ldwb, Db, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1}, (T*)dX, lddx, M, K, jx, "gated_ffn_dx")) return rc;
-    if (dW)
-      if (int rc = product(std::true_type{}, need.pw, Args{(const char*)D, Xr, need.ldd * es, ldxb, Db, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, 1}, (T*)dW, K, 2 * H, K, jw, "gated_ffn_dw")) return rc;
+      if (int rc = product(std::false_type{}, std::false_type{}, need.px,
+                           Args{(const char*)D, Wr, need.ldd * es, ldwb, Db, (2 * H - 1) * ldwb + kb, 0, (int)(2 * H), 0, 0, 0, 1},
+                           dX, lddx, M, K, jx, "gated_ffn_dx")) return rc;
+    if (dW) {
+      const Args a{(const char*)D, Xr, need.ldd * es, ldxb, Db, (M - 1) * ldxb + kb, 0, (int)M, 0, 0, 0, 1};
+      if (int rc = add_w ? product(std::true_type{}, std::true_type{}, need.pw, a, dW, K, 2 * H, K, jw, "gated_ffn_dw")
+                         : product(std::true_type{}, std::false_type{}, need.pw, a, dW, K, 2 * H, K, jw, "gated_ffn_dw")) return rc;
+    }
     return join(sums, rowblocks);
   });
+}
+
+extern "C" int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre,
+                                 const void* dH, long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K,
+                                 int act, void* ws, long ws_bytes, void* stream) {
+  return backward(dtype, X, ldx, W, ldw, pre, dH, lddh, dX, lddx, dW, db, 0, M, H, K, act, ws, ws_bytes, stream);
+}
+
+extern "C" int svk_gated_ffn_bwd_add(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre,
+                                     const void* dH, long lddh, void* dX, long lddx, void* dW, float* db, int add, long M,
+                                     long H, long K, int act, void* ws, long ws_bytes, void* stream) {
+  if (add & ~(SVK_ADD_DW | SVK_ADD_DB)) { set_error("svk_gated_ffn_bwd: unknown bits in add"); return SVK_EINVAL; }
+  return backward(dtype, X, ldx, W, ldw, pre, dH, lddh, dX, lddx, dW, db, add, M, H, K, act, ws, ws_bytes, stream);
 }

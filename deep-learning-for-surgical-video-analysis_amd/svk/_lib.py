@@ -117,6 +117,8 @@ SIGNATURES = {
     "svk_gated_ffn": [c_int, P, c_long, P, c_long, P, P, c_long, P, c_long, c_long, c_long, c_int, P, c_long, P],
     "svk_gated_ffn_bwd": [c_int, P, c_long, P, c_long, P, P, c_long, P, c_long, P, P, c_long, c_long, c_long, c_int, P,
                           c_long, P],
+    "svk_gated_ffn_bwd_add": [c_int, P, c_long, P, c_long, P, P, c_long, P, c_long, P, P, c_int, c_long, c_long, c_long, c_int,
+                              P, c_long, P],
     "svk_quant_rows": [c_int, P, c_long, P, c_long, P, c_long, c_long, P],
     "svk_gemm_i8": [c_int, P, c_long, P, P, c_long, P, P, P, c_long, P, c_long, c_long, c_long, c_long, c_int, P, c_long,
                     P],

@@ -1734,9 +1734,22 @@ def gated_ffn(x, w, bias=None, act="silu", save=False, out=None):
     return (out, pre) if save else out
 
 
+def _given(g, shape, dev, fn, name, *others):
+    """(the buffer to add to, or None; whether the gradient is wanted) of a dw / db argument."""
+    if not torch.is_tensor(g):
+        return None, bool(g)
+    _like(g, torch.float32, dev, fn, name)
+    if g.shape != shape or not g.is_contiguous():
+        raise _lib.SvkError(f"svk.{fn}: {name} to add to must be contiguous float32 {tuple(shape)}, got {tuple(g.shape)}")
+    if not all(_apart(g, t, same=False) for t in others):
+        raise _lib.SvkError(f"svk.{fn}: {name} to add to overlaps an input or the other gradient")
+    return g, True
+
+
 def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
     """Gradients (dx, dw, db) of gated_ffn from dh [..., hidden] and the saved ``pre``: dx like x, dw [2 * hidden, K] in
     w's dtype, db float32 [2 * hidden]; None where not asked for.  Written, not added to; the same bits on every run.
+    A float32 tensor as ``dw`` / ``db`` is added to instead, in float32, and returned (gradient buffers, as gemm_wgrad's).
     The gradients of the projections are rounded once to x's dtype before the two products (db sums them unrounded);
     float32 operands keep them in 32 bits."""
     fn = "gated_ffn_bwd"
@@ -1750,18 +1763,20 @@ def gated_ffn_bwd(x, w, pre, dh, act="silu", dx=True, dw=True, db=True):
     if dh.shape != (*lead, H):
         raise _lib.SvkError(f"svk.{fn}: dh {tuple(dh.shape)} is not {(*lead, H)}")
     _, _, lddh = _token_rows(dh, fn, "dh")
+    aw, dw = _given(dw, (2 * H, K), dev, fn, "dw", x, w, pre, dh)
+    ab, db = _given(db, (2 * H,), dev, fn, "db", x, w, pre, dh, aw)
     gx = torch.empty((*lead, K), device=x.device, dtype=x.dtype) if dx else None
-    gw = torch.empty((2 * H, K), device=x.device, dtype=x.dtype) if dw else None
-    gb = torch.empty(2 * H, device=x.device, dtype=torch.float32) if db else None
+    gw = aw if aw is not None or not dw else torch.empty((2 * H, K), device=x.device, dtype=x.dtype)
+    gb = ab if ab is not None or not db else torch.empty(2 * H, device=x.device, dtype=torch.float32)
     if M and (dx or dw or db):
         lib, px, pw = _lib.load(), x.data_ptr(), w.data_ptr()
         nb = lib.svk_gated_ffn_bwd_workspace(dt, px, ldx, pw, ldw, M, H, K, 1 if dx else 0, 1 if dw else 0, 1 if db else 0)
         ws = torch.empty(nb, device=x.device, dtype=torch.uint8)
-        _on(dev, lib.svk_gated_ffn_bwd, dt, px, ldx, pw, ldw, pre.data_ptr(), dh.data_ptr(), lddh, _p(gx), K, _p(gw), _p(gb),
-            M, H, K, code, ws.data_ptr(), nb)
+        _on(dev, lib.svk_gated_ffn_bwd_add, dt, px, ldx, pw, ldw, pre.data_ptr(), dh.data_ptr(), lddh, _p(gx), K, _p(gw), _p(gb),
+            (aw is not None) + 2 * (ab is not None), M, H, K, code, ws.data_ptr(), nb)
     elif M == 0:
-        for t in (gw, gb):
-            if t is not None:
+        for t, given in ((gw, aw), (gb, ab)):
+            if t is not None and given is None:
                 t.zero_()
     return gx, gw, gb
 

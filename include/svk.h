@@ -33,6 +33,7 @@ extern "C" {
 enum { SVK_F32 = 0, SVK_BF16 = 1, SVK_F16 = 2 };
 enum { SVK_ACT_NONE = 0, SVK_ACT_GELU = 1, SVK_ACT_RELU = 2, SVK_ACT_TANH = 3 };
 enum { SVK_GLU_SILU = 0, SVK_GLU_GELU = 1, SVK_GLU_RELU = 2 };      /* activation of svk_gated_ffn's gate */
+enum { SVK_ADD_DW = 1, SVK_ADD_DB = 2 };                             /* svk_gated_ffn_bwd_add */
 enum { SVK_POS_I32 = 0, SVK_POS_I64 = 1, SVK_POS_F32 = 2 };          /* type of svk_rope3d's positions */
 enum { SVK_OK = 0, SVK_EINVAL = -1, SVK_EUNSUPPORTED = -2, SVK_ELAUNCH = -3 };
 
@@ -623,6 +624,12 @@ long svk_gated_ffn_bwd_workspace(int dtype, const void* X, long ldx, const void*
 int svk_gated_ffn_bwd(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH,
                       long lddh, void* dX, long lddx, void* dW, float* db, long M, long H, long K, int act, void* ws,
                       long ws_bytes, void* stream);
+/* The same with gradients that are added to, as svk_gemm_wgrad's: with SVK_ADD_DW in `add` dW is f32 [2H, K] contiguous and
+ * receives += the f32 sums, with SVK_ADD_DB db receives += its sums (M = 0 leaves them as they are); a gradient without its
+ * bit is written as above.  The same workspace. */
+int svk_gated_ffn_bwd_add(int dtype, const void* X, long ldx, const void* W, long ldw, const void* pre, const void* dH,
+                          long lddh, void* dX, long lddx, void* dW, float* db, int add, long M, long H, long K, int act,
+                          void* ws, long ws_bytes, void* stream);
 /* Host query: which tiles a product runs on.  product 0: the forward pass [M, 2H], 1: dX [M, K], 2: dW [2H, K].
  * plan[4] = side of the square tiles (0: the few-token kernel), parts its reduction is split into, rows of the result that
  * they cover, side of the tiles of the rows behind (0: none). */

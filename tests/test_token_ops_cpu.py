@@ -267,3 +267,26 @@ def test_plan_queries():
     for bad in ((1, 3, 8, 8, 8), (1, -1, 8, 8, 8), (9, 0, 8, 8, 8), (1, 0, 0, 8, 8), (1, 0, 8, 0, 8), (1, 0, 8, 8, -1)):
         assert lib.svk_gated_ffn_plan(*bad, p) == -1
     assert lib.svk_gated_ffn_plan(1, 0, 8, 8, 8, None) == -1 and lib.svk_gemm_i8_plan(8, 8, 131072, p) == -1
+
+
+def test_gradient_buffers_to_add_to():
+    import svk
+    from svk import ops
+    x, w = torch.zeros(6, 16), torch.zeros(8, 16)
+    dw, db = torch.zeros(8, 16), torch.zeros(8)
+    f = lambda g, *others: ops._given(g, (8, 16), -1, "f", "dw", *others)  # noqa: E731
+    assert f(True) == (None, True) and f(False) == (None, False) and f(None) == (None, False) and f(1) == (None, True)
+    assert f(dw, x, w, None, db)[0] is dw and f(dw, x)[1] is True
+    flat = torch.zeros(8 * 16 + 8)
+    assert f(flat[:128].view(8, 16), flat[128:])[1] is True
+    for bad, others in ((dw.half(), ()), (dw[:7], ()), (dw.flatten(), ()), (torch.zeros(16, 8).t(), ()), (torch.zeros(8, 32)[:, :16], ()),
+                        (w, (x, w)), (flat[:128].view(8, 16), (flat[120:128],)), (flat[8:].view(8, 16), (flat[:16],))):
+        with pytest.raises(svk.SvkError, match="dw"):
+            f(bad, *others)
+
+
+@pytest.mark.parametrize("add", [4, -1, 8])
+def test_gated_ffn_bwd_add_refuses(add):
+    lib = _lib()
+    rc = lib.svk_gated_ffn_bwd_add(0, A, 64, A, 64, A, A, 32, A, 64, A, A, add, 100, 32, 64, 0, A, 1 << 30, None)
+    assert rc == -1 and b"add" in lib.svk_last_error()

@@ -358,6 +358,78 @@ def test_gated_ffn_bwd_products_past_the_range_behind_closed_gates(cuda):
                 assert not bool(t.any())
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("M,H,K", [(1, 1, 1), (7, 33, 50), (200, 853, 320), (1000, 96, 61), (4874, 33, 1043), (16640, 256, 512),
+                                   (833, 2505, 803), (325, 4734, 1797), (4357, 365, 650)])
+def test_gated_ffn_bwd_added_to_gradient_buffers(cuda, dt, M, H, K):
+    """dw and db added to f32 buffers, in f32: the sums (to 4 M) are exact, whatever the type would round them to.  What
+    lies around the buffers stays."""
+    ops = _ops()
+    x, w = _ints(M, K, dt=dt, seed=4), _ints(2 * H, K, dt=dt, seed=5)
+    pre, dh = _ints(M, 2 * H, dt=dt, seed=6, top=2), _ints(M, H, dt=dt, seed=7, top=2)
+    g, u, d = pre[:, :H].to(F64), pre[:, H:].to(F64), dh.to(F64)
+    dp = torch.cat([d * u * (g > 0), d * torch.relu(g)], 1)
+    dw, db = dp.t().contiguous() @ x.to(F64), dp.sum(0)
+    n = 2 * H * K
+    flat = torch.full((n + 2 * H + 12,), 5.0, device="cuda")                 # a flat buffer of gradients, at an odd place
+    gw, gb = flat[3:3 + n].view(2 * H, K), flat[3 + n + 4:3 + n + 4 + 2 * H]
+    start = _ints(2 * H, K, dt=torch.float32, seed=8, top=9000)
+    gw.copy_(start)
+    gb.copy_(start[:, 0])
+    for turn in (1, 2):
+        dx, rw, rb = ops.gated_ffn_bwd(x, w, pre, dh, act="relu", dw=gw, db=gb)
+        assert rw is gw and rb is gb
+        assert torch.equal(gw.to(F64), start.to(F64) + turn * dw) and torch.equal(gb.to(F64), start[:, 0].to(F64) + turn * db)
+        assert torch.equal(dx, (dp @ w.to(F64)).float().to(dt))
+    assert bool((flat[:3] == 5).all()) and bool((flat[3 + n:3 + n + 4] == 5).all()) and bool((flat[3 + n + 4 + 2 * H:] == 5).all())
+    # one of them added to, the other written
+    gb.zero_()
+    _, w16, rb = ops.gated_ffn_bwd(x, w, pre, dh, act="relu", dx=False, db=gb)
+    assert rb is gb and torch.equal(gb.to(F64), db) and w16.dtype == dt and torch.equal(w16, dw.float().to(dt))
+    gw.zero_()
+    _, rw, rb = ops.gated_ffn_bwd(x, w, pre, dh, act="relu", dw=gw)
+    assert torch.equal(gw.to(F64), dw) and torch.equal(rb.to(F64), db)
+    # no tokens: nothing is added
+    ops.gated_ffn_bwd(x[:0], w, pre[:0], dh[:0], act="relu", dw=gw, db=gb)
+    assert torch.equal(gw.to(F64), dw) and torch.equal(gb.to(F64), db)
+
+
+def test_gated_ffn_bwd_entry_adds_nothing_without_tokens(cuda):
+    from svk import _lib
+    lib = _lib.load()
+    x, w = torch.zeros(1, 16, device="cuda"), torch.zeros(24, 16, device="cuda")
+    dw, db = torch.ones(24, 16, device="cuda"), torch.ones(24, device="cuda")
+    p, st = x.data_ptr(), torch.cuda.current_stream().cuda_stream
+    for add, left in ((3, (1, 1)), (1, (1, 0)), (2, (0, 1))):
+        dw.fill_(1)
+        db.fill_(1)
+        assert lib.svk_gated_ffn_bwd_add(0, p, 16, w.data_ptr(), 16, p, p, 12, p, 16, dw.data_ptr(), db.data_ptr(), add, 0, 12,
+                                         16, 0, None, 0, st) == 0
+        torch.cuda.synchronize()
+        assert bool((dw == left[0]).all()) and bool((db == left[1]).all())
+
+
+def test_gated_ffn_bwd_added_to_buffers_in_a_graph(cuda):
+    """Captured: every replay adds once more; eager calls between them too."""
+    ops = _ops()
+    M, H, K, dt = 3000, 40, 72, torch.bfloat16
+    x, w = _ints(M, K, dt=dt, seed=4), _ints(2 * H, K, dt=dt, seed=5)
+    pre, dh = _ints(M, 2 * H, dt=dt, seed=6, top=2), _ints(M, H, dt=dt, seed=7, top=2)
+    _, one, oneb = ops.gated_ffn_bwd(x.float(), w.float(), pre.float(), dh.float(), act="relu")
+    gw, gb = torch.zeros(2 * H, K, device="cuda"), torch.zeros(2 * H, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.gated_ffn_bwd(x, w, pre, dh, act="relu", dw=gw, db=gb)
+    n = 0
+    for _ in range(3):
+        g.replay()
+        ops.gated_ffn_bwd(x, w, pre, dh, act="relu", dx=False, dw=gw, db=gb)
+        n += 2
+        torch.cuda.synchronize()
+        assert torch.equal(gw, n * one) and torch.equal(gb, n * oneb)
+
+
 def test_gated_ffn_gradient_against_differences(cuda):
     """f32: the derivative of sum(h * dh) along random directions of x, w and the bias, by central differences of the
     forward kernel.  Steps of 2^-6: third-order term ~ 2^-12 of the slope's scale, rounding ~ 2^-24 / 2^-6."""
