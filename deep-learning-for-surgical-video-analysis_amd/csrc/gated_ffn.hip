@@ -493,7 +493,7 @@ static int backward(int dtype, const void* X, long ldx, const void* W, long ldw,
     auto blocks_of = [](long values) { return (int)std::min<long>((values + 256 * JOIN - 1) / (256 * JOIN), 4096); };
     Slabs jx{};
     Slabs jw{};
-    const int db_blocks = db ? (int)((2 * H + 15) / 16) : 0;
+    const int db_blocks = db && (M || !add_b) ? (int)((2 * H + 15) / 16) : 0;
     auto join = [&](const float* sums, int rows) -> int {
       const int all = jx.blocks + jw.blocks + db_blocks;
       if (!all) return SVK_OK;

@@ -12,6 +12,7 @@
 // Bound by HBM: q and k are read once and written once, as 16-byte pieces.
 #include "svk_common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace svk {
 namespace rope {
@@ -46,6 +47,14 @@ __device__ __forceinline__ void get(const T* p, int n, float* v) {
     for (int e = 0; e < V; ++e) v[e] = e < n ? to_f(p[e]) : 0.f;
   }
 }
+// A value's last rounding in f32, kept apart from the conversion: the compiler fuses the two into one instruction with one
+// rounding (v_fma_mixlo_f16) for some of a piece's pairs and not for others, and a pair's bits must not depend on where it
+// lies (pieces overlap).  The same time.
+template <typename T>
+__device__ __forceinline__ float rounded(float v) {
+  if constexpr (std::is_same<T, f16>::value) asm("" : "+v"(v));
+  return v;
+}
 template <typename T, int V>
 __device__ __forceinline__ void set(T* p, int n, const float* v) {
   typedef T vec __attribute__((ext_vector_type(V)));
@@ -53,12 +62,12 @@ __device__ __forceinline__ void set(T* p, int n, const float* v) {
   if (n >= V) {
     vec w;
 #pragma unroll
-    for (int e = 0; e < V; ++e) w[e] = from_f<T>(v[e]);
+    for (int e = 0; e < V; ++e) w[e] = from_f<T>(rounded<T>(v[e]));
     *reinterpret_cast<anywhere*>(p) = w;
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (e < n) p[e] = from_f<T>(v[e]);
+      if (e < n) p[e] = from_f<T>(rounded<T>(v[e]));
   }
 }
 

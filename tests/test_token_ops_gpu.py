@@ -155,6 +155,25 @@ def test_rope3d_time_major_in_place(cuda, dt):
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, keep)
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("hd,sections", [(59, (8, 1, 18)), (24, (3, 3, 3)), (40, (6, 6, 7))])
+def test_rope3d_bits_do_not_depend_on_the_piece(cuda, dt, il, hd, sections):
+    """A pair is rounded alike wherever it lies in a 16-byte piece: pieces overlap at the end of a part of odd length (both
+    write the same bits then, in any order), and in place they do not overlap."""
+    ops = _ops()
+    B, N, h = 6, 1500, 4
+    q = _rand(B, N, h * hd, dt=dt, seed=9)
+    pos = torch.randint(0, 5000, (N, 3), generator=torch.Generator().manual_seed(1)).cuda()
+    f = ops.rope3d_freqs(sections)
+    first = ops.rope3d(q, None, pos, f, sections, h, interleaved=il)[0]
+    for _ in range(3):
+        assert torch.equal(ops.rope3d(q, None, pos, f, sections, h, interleaved=il)[0], first)
+    _rope_close(first, q, pos, f, sections, h, il, False)
+    ops.rope3d(q, None, pos, f, sections, h, interleaved=il, out=(q, None))
+    assert torch.equal(q, first)
+
+
 def test_rope3d_positions_that_are_not_finite(cuda):
     ops = _ops()
     q = torch.ones(1, 2, 8, device="cuda")
